@@ -117,7 +117,7 @@ __device__ __forceinline__ void lds_bias(f32x4 (&bias)[TM], const float* bias_s,
     for (int tm = 0; tm < TM; ++tm) bias[tm] = *(const f32x4*)(bias_s + conv * C + chl + 4 * tm);
 }
 
-// leaky_relu on 4 values as max(x, slope*x) (0 < slope <= 1): two packed multiplies + four v_max
+// leaky_relu on 4 values as max(x, slope*x) (0 < slope <= 1): four multiplies + four v_max
 __device__ __forceinline__ f32x4 lrelu4(const f32x4& v, float slope) {
     const f32x4 s = v * slope;
     return f32x4{fmaxf(v[0], s[0]), fmaxf(v[1], s[1]), fmaxf(v[2], s[2]), fmaxf(v[3], s[3])};

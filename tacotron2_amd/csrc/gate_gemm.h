@@ -98,8 +98,8 @@ __device__ __forceinline__ void glds16(const void* src, char* lds_dst) {
                                      (__attribute__((address_space(3))) void*)lds_dst, 16, 0, 0);
 }
 
-// gate_act<true> (conv_mfma.h) on two values at a time: the multiplies and adds around the three transcendentals as
-// packed fp32 operations (the epilogue is VALU-bound: 64 gates per lane, two waves per SIMD)
+// gate_act<true> (conv_mfma.h) on two values at a time (the epilogue is VALU-bound: 64 gates per lane, two waves per SIMD;
+// the build keeps hipcc from making packed fp32 instructions of the pairs)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 gate_act_x2(f32x2 t, f32x2 s) {
     constexpr float kLog2e = 1.44269504088896341f;
