@@ -220,6 +220,97 @@ MV_API void mv_destroy(mv_handle h);
  * device buffer of n samples, on device. */
 MV_API int mv_pcm16(const float* wav, size_t n, int16_t* pcm, void* stream);
 
+/* ---- sequence operators: layers on channels-last tensors -----------------------------------
+ * No counterpart in the reference, whose models hold none of these layers: they are what an acoustic or vocoder model
+ * built beside this library's convolutions needs -- group normalisation with its activation, the short causal depthwise
+ * convolution and the selective state space scan, the last two for prompts and for single frames (state in, state out).
+ *
+ * A tensor is [B][T][C] with adjacent channels and any batch and row stride (mv_rows; strides in elements, so halves of a
+ * projection's output or [T][B][C] memory are taken as they lie).  Data are float32, bfloat16 or float16 (`dtype`),
+ * arithmetic is float32 with one rounding at the store; float16 results beyond its range become infinities.  `lengths` is a
+ * device int32 [B] of true frame counts or NULL (all T); entries are clamped into [0, T] by the kernels.  Frames at or past
+ * a sequence's end are never read into a result and are written as 0.  Calls run on the current HIP device, are
+ * asynchronous on `stream`, allocate nothing and may be captured; the caller owns every buffer.  Outputs must not overlap
+ * inputs except where an entry says so.  B = 0 or T = 0 is a call with nothing to do. */
+#define MV_DTYPE_F32 0
+#define MV_DTYPE_BF16 1
+#define MV_DTYPE_F16 2
+
+#define MV_ACT_NONE 0
+#define MV_ACT_SILU 1  /* v * sigmoid(v) */
+#define MV_ACT_LRELU 2 /* v < 0 ? slope * v : v; slope 0 is relu */
+#define MV_ACT_TANH 3
+
+typedef struct mv_rows {
+    void* ptr;            /* element (b, t, c) at ptr + (b * batch_stride + t * row_stride + c) elements */
+    int64_t batch_stride; /* elements */
+    int64_t row_stride;   /* elements */
+} mv_rows;
+
+/* y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and (biased) variance of each group of C / groups adjacent
+ * channels: over all of a sequence's true frames, or (per_frame) over each frame by itself, which is the form a stream can
+ * use.  y may be x itself (same pointer and strides). */
+typedef struct mv_group_norm_args {
+    mv_rows x, y;
+    const void* weight;     /* [C] or NULL (1) */
+    const void* bias;       /* [C] or NULL (0) */
+    const int32_t* lengths; /* [B] or NULL */
+    int B, T, C, groups;
+    int dtype;          /* MV_DTYPE_* of x and y */
+    int weight_dtype;   /* MV_DTYPE_* of weight and bias: MV_DTYPE_F32 or dtype */
+    int per_frame;      /* 0: statistics per sequence, 1: per frame */
+    int activation;     /* MV_ACT_* */
+    float slope;        /* of MV_ACT_LRELU */
+    float eps;          /* >= 0 */
+} mv_group_norm_args;
+/* scratch of mv_group_norm in bytes (256-byte aligned; 0: none needed, workspace may be NULL) */
+MV_API size_t mv_group_norm_workspace(const mv_group_norm_args* a);
+MV_API int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[t, c] = act(bias[c] + sum_k weight[c, k] * x[t - K + 1 + k, c]): each channel by itself, frame t sees frames up to t.
+ * Frames before the first come from `state_in` (the K - 1 frames before, oldest first; NULL: zeros), and `state_out` (or
+ * NULL) gets the last K - 1 frames of (state_in, x[:lengths[b]]): a sequence cut into calls gives the results of one call.
+ * state_out may be state_in itself; y may not be x. */
+typedef struct mv_causal_conv_args {
+    mv_rows x, y;
+    const void* weight;     /* [C][K] */
+    const void* bias;       /* [C] or NULL */
+    const void* state_in;   /* [B][K - 1][C], contiguous, of dtype, or NULL */
+    void* state_out;        /* [B][K - 1][C], contiguous, of dtype, or NULL */
+    const int32_t* lengths; /* [B] or NULL */
+    int B, T, C, K;         /* 1 <= K <= 8 */
+    int dtype;              /* MV_DTYPE_* of x, y and the states */
+    int weight_dtype;       /* MV_DTYPE_F32 or dtype */
+    int activation;         /* MV_ACT_* */
+    float slope;            /* of MV_ACT_LRELU */
+} mv_causal_conv_args;
+MV_API int mv_causal_conv(const mv_causal_conv_args* a, void* stream);
+
+/* The state space recurrence of D channels with N states each, whose step, input and output maps come from the data:
+ *   dt = delta + delta_bias, softplus of it if delta_softplus
+ *   h[n] = exp(dt * A[d, n]) * h[n] + dt * u * B[g, n]
+ *   y = (sum_n C[g, n] * h[n] + Dskip[d] * u) * (z * sigmoid(z) if z)
+ * per frame, with g = d / (D / G).  h starts from `state_in` (NULL: zeros) and its value after the last true frame goes to
+ * `state_out` (or NULL); state_out may be state_in itself.  States are float32. */
+typedef struct mv_selective_scan_args {
+    mv_rows u, delta, z; /* [B][T][D]; z.ptr NULL: no gate */
+    mv_rows Bm, Cm;      /* [B][T][G][N], groups `Bg_stride` / `Cg_stride` elements apart */
+    int64_t Bg_stride, Cg_stride;
+    mv_rows y;               /* [B][T][D] */
+    const float* A;          /* [D][N] */
+    const float* Dskip;      /* [D] or NULL */
+    const float* delta_bias; /* [D] or NULL */
+    const float* state_in;   /* [B][D][N] contiguous or NULL */
+    float* state_out;        /* [B][D][N] contiguous or NULL */
+    const int32_t* lengths;  /* [B] or NULL */
+    int B, T, D, N, G;       /* 1 <= N <= 64, D a multiple of G */
+    int dtype;               /* MV_DTYPE_* of u, delta, z, Bm, Cm and y */
+    int delta_softplus;
+} mv_selective_scan_args;
+/* scratch of mv_selective_scan in bytes (256-byte aligned; 0: none needed, workspace may be NULL) */
+MV_API size_t mv_selective_scan_workspace(const mv_selective_scan_args* a);
+MV_API int mv_selective_scan(const mv_selective_scan_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- measurement: per-launch HIP-event timing of the MFMA kernels (bench.py's roofline figure).
  * No counterpart in the reference.  After mv_profile_begin(h) every convolution launch of the
  * following forward/infer calls is bracketed by hipEventRecord on the call's stream;

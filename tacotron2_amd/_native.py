@@ -25,6 +25,7 @@ EXPORTS = (
     "mv_waveglow_infer", "mv_workspace_bytes", "mv_hop", "mv_macs_per_frame", "mv_destroy", "mv_pcm16",
     "mv_test_conv1d", "mv_test_conv_transpose1d", "mv_profile_begin", "mv_profile_end",
     "mv_postnet_create", "mv_postnet_forward", "mv_default_options", "mv_hifigan_forward_static",
+    "mv_group_norm", "mv_group_norm_workspace", "mv_causal_conv", "mv_selective_scan", "mv_selective_scan_workspace",
 )
 STATIC_SCRATCH_BYTES = 64 << 20  # MV_STATIC_SCRATCH_BYTES
 
@@ -70,6 +71,33 @@ class mv_postnet_cfg(C.Structure):
 
 class mv_options(C.Structure):
     _fields_ = [("fuse", C.c_int), ("io16", C.c_int), ("wg_fold", C.c_int), ("wg_gemm", C.c_int)]
+
+
+def _rows(name):
+    """The fields of an mv_rows, in place: a flat structure is filled by one positional call."""
+    return [(name, C.c_void_p), (name + "_batch_stride", C.c_int64), (name + "_row_stride", C.c_int64)]
+
+
+def _fields(kind, names):
+    return [(n, kind) for n in names.split()]
+
+
+class mv_group_norm_args(C.Structure):
+    _fields_ = (_rows("x") + _rows("y") + _fields(C.c_void_p, "weight bias lengths")
+                + _fields(C.c_int, "B T C groups dtype weight_dtype per_frame activation")
+                + _fields(C.c_float, "slope eps"))
+
+
+class mv_causal_conv_args(C.Structure):
+    _fields_ = (_rows("x") + _rows("y") + _fields(C.c_void_p, "weight bias state_in state_out lengths")
+                + _fields(C.c_int, "B T C K dtype weight_dtype activation") + [("slope", C.c_float)])
+
+
+class mv_selective_scan_args(C.Structure):
+    _fields_ = (_rows("u") + _rows("delta") + _rows("z") + _rows("Bm") + _rows("Cm")
+                + _fields(C.c_int64, "Bg_stride Cg_stride") + _rows("y")
+                + _fields(C.c_void_p, "A Dskip delta_bias state_in state_out lengths")
+                + _fields(C.c_int, "B T D N G dtype delta_softplus"))
 
 
 def make_options(options):
@@ -138,6 +166,11 @@ def lib():
     l.mv_pcm16.argtypes = [vp, C.c_size_t, vp, vp]
     l.mv_test_conv1d.argtypes = [vp, vp, i32, i32, i32, f32p, f32p, i32, i32, i32, C.c_float, i32, vp, vp]
     l.mv_test_conv_transpose1d.argtypes = [vp, vp, i32, i32, i32, f32p, f32p, i32, i32, i32, i32, C.c_float, i32, vp, vp]
+    for fn, args in (("mv_group_norm", mv_group_norm_args), ("mv_selective_scan", mv_selective_scan_args)):
+        getattr(l, fn).argtypes = [C.POINTER(args), vp, C.c_size_t, vp]
+        getattr(l, fn + "_workspace").argtypes = [C.POINTER(args)]
+        getattr(l, fn + "_workspace").restype = C.c_size_t
+    l.mv_causal_conv.argtypes = [C.POINTER(mv_causal_conv_args), vp]
     l.mv_profile_begin.argtypes = [vp]
     l.mv_profile_end.argtypes = [vp, C.POINTER(mv_profile_row), i32, C.POINTER(i32)]
     _lib = l

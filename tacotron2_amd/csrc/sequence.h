@@ -1,0 +1,107 @@
+// sequence.h -- what the sequence operators share (group_norm.hip, causal_conv.hip, selective_scan.hip): element types,
+// activations, row addressing.  The operators work on channels-last tensors [B][T][C] whose channels are adjacent and
+// whose rows and batches lie at any stride (mv_rows); arithmetic is float32, one rounding at the store.
+#pragma once
+#include "common.h"
+
+namespace mv {
+
+// one tensor of a launch: element (b, t, c) at ptr + b * bs + t * rs + c
+template <typename T>
+struct Rows {
+    T* p;
+    long long bs, rs;
+    __device__ __forceinline__ T* row(int b, int t) const { return p + b * bs + t * rs; }
+};
+template <typename T>
+inline Rows<T> rows_of(const mv_rows& r) {
+    return Rows<T>{(T*)r.ptr, (long long)r.batch_stride, (long long)r.row_stride};
+}
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// sigmoid and its relatives on the hardware exp2 and reciprocal (1 ulp each): exp2 overflowing to inf gives the right 0
+__device__ __forceinline__ float sigmoidf(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+// tanh: (1 - e) / (1 + e) with e = exp(-2|x|) loses x's low bits near 0, where the Taylor series to x^9 takes over
+// (its next term is under 1e-8 of the result at 1/4)
+__device__ __forceinline__ float tanh_accurate(float x) {
+    const float a = fabsf(x);
+    if (a < 0.25f) {
+        const float q = x * x;
+        return x * (1.f + q * (-1.f / 3 + q * (2.f / 15 + q * (-17.f / 315 + q * (62.f / 2835)))));
+    }
+    const float e = __builtin_amdgcn_exp2f(-2.f * kLog2e * a);
+    return copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+}
+
+// the activations of mv_group_norm and mv_causal_conv; a NaN stays a NaN, relu (slope 0) takes -inf to 0
+template <int ACT>
+__device__ __forceinline__ float activate(float v, float slope) {
+    if (ACT == MV_ACT_SILU) return v * sigmoidf(v);
+    if (ACT == MV_ACT_LRELU) return v < 0.f ? (slope == 0.f ? 0.f : slope * v) : v;
+    if (ACT == MV_ACT_TANH) return tanh_accurate(v);
+    return v;
+}
+
+// weights are float32 or of the data's type
+template <typename T>
+__device__ __forceinline__ float load_weight(const void* w, bool w32, int i) {
+    return w32 ? ((const float*)w)[i] : (float)((const T*)w)[i];
+}
+
+// calls f with a value of the element type / of an integral_constant for the activation
+template <typename F>
+inline int by_dtype(int dtype, F&& f) {
+    switch (dtype) {
+        case MV_DTYPE_F32: return f(float());
+        case MV_DTYPE_BF16: return f(__bf16());
+        case MV_DTYPE_F16: return f(_Float16());
+    }
+    set_error("unknown dtype %d", dtype);
+    return MV_EINVAL;
+}
+template <typename F>
+inline int by_activation(int act, F&& f) {
+    switch (act) {
+        case MV_ACT_NONE: return f(std::integral_constant<int, MV_ACT_NONE>());
+        case MV_ACT_SILU: return f(std::integral_constant<int, MV_ACT_SILU>());
+        case MV_ACT_LRELU: return f(std::integral_constant<int, MV_ACT_LRELU>());
+        case MV_ACT_TANH: return f(std::integral_constant<int, MV_ACT_TANH>());
+    }
+    set_error("unknown activation %d", act);
+    return MV_EINVAL;
+}
+
+inline size_t dtype_size(int dtype) { return dtype == MV_DTYPE_F32 ? 4 : 2; }
+
+// rows of an output must not overlap: batches of rows, or rows of batches ([T][B][C] memory)
+inline bool rows_disjoint(const mv_rows& r, int B, int T, int C) {
+    const int64_t b = r.batch_stride, t = r.row_stride;
+    return ((T < 2 || t >= C) && (B < 2 || b >= (T - 1) * t + C)) || ((B < 2 || b >= C) && (T < 2 || t >= (B - 1) * b + C));
+}
+
+// a call without frames: the sequences stand where they stood
+template <typename T>
+__global__ __launch_bounds__(256) void carry_state_kernel(const T* in, T* out, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
+        out[i] = in ? in[i] : (T)0.f;
+}
+template <typename T>
+inline int carry_state(const T* in, T* out, long long n, hipStream_t stream) {
+    if (!out || in == out || n == 0) return MV_OK;
+    const long long blocks = (n + 255) / 256;
+    hipLaunchKernelGGL((carry_state_kernel<T>), dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, stream, in,
+                       out, n);
+    MV_HIP(hipGetLastError());
+    return MV_OK;
+}
+
+// host-side checks shared by the operators; `who` is the entry point's name
+int check_sequence(const char* who, int B, int T, int C, int dtype);
+int check_rows(const char* who, const char* what, const mv_rows& r, int dtype);
+int check_states(const char* who, const void* in, const void* out, long long bytes);
+int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, int dtype);
+
+}  // namespace mv

@@ -1,0 +1,695 @@
+"""The sequence operators (tacotron2_amd.sequence) on the GPU against plain float64 restatements.
+
+Tolerances.  A result is held to half a step of its type (eps / 2 of its value) plus the float32 error of what led to it,
+which each reference computes beside the value by running error analysis with u = 2^-24 (half a float32 step): a sum or a
+product of floats adds u of its value; the hardware exp2, reciprocal and the division built on it are good to 1 ulp = 2u.
+float16 results additionally get half the smallest subnormal (2^-25), bfloat16 and float32 results 1e-37 (subnormals
+flushed)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tacotron2_amd import _native, sequence  # noqa: E402
+
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _rng(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _near(got, want, err, what=""):
+    """|got - want| <= half a step of got's type + err, element by element; want and err are float64 on the CPU."""
+    got = got.detach().cpu()
+    tiny = 2.0 ** -25 if got.dtype == F16 else 1e-37
+    half = torch.finfo(got.dtype).eps / 2
+    d = (got.double() - want).abs()
+    tol = half * (want.abs() + err) + err + tiny
+    bad = ~(d <= tol)
+    assert not bad.any(), (what, "worst", float((d / tol).max()), "at", [int(i) for i in bad.nonzero()[0]],
+                           "of", list(got.shape), "bad", int(bad.sum()))
+
+
+def _activate(v, err, act, slope=0.1):
+    """(act(v), its error): silu' <= 1.1, tanh' <= 1; exp's argument is rounded (|v| u in e), then exp, sum, reciprocal and
+    product: 2 + 1 + 2 + 1 roundings of the result."""
+    if act == "silu":
+        s = torch.sigmoid(v)
+        return v * s, 1.1 * err + (8 + 2 * v.abs() * (1 - s)) * U * (v * s).abs()
+    if act == "tanh":  # near zero the series is good to 8 u, beyond a quarter 1 - e keeps two bits at least
+        return torch.tanh(v), err + 24 * U * torch.tanh(v).abs()
+    if act == "relu":
+        return v.clamp(min=0), err
+    if act == "leaky_relu":
+        return torch.where(v < 0, slope * v, v), err + 2 * U * slope * v.abs()
+    return v, err
+
+
+def _ends(lengths, B, T):
+    return [T] * B if lengths is None else [min(max(int(n), 0), T) for n in lengths]
+
+
+def _on(lengths):
+    return None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+
+# --- group norm ----------------------------------------------------------------------------------------------------
+def norm_ref(x, G, w, b, eps, act, per_frame, ends):
+    """(y, error).  The mean of n floats summed in any order of at most `depth` additions a path is off by depth * u *
+    mean|x|; x - m by that and one rounding; the variance's error is relative (the squares add up with one sign) and counts
+    half in the root: r is off by (depth + 8) / 2 * u + what the mean's error puts in, which is of second order."""
+    B, T, C = x.shape
+    y, e = torch.zeros(B, T, C, dtype=torch.float64), torch.zeros(B, T, C, dtype=torch.float64)
+    wd = torch.ones(C, dtype=torch.float64) if w is None else w.double()
+    bd = torch.zeros(C, dtype=torch.float64) if b is None else b.double()
+    for i, end in enumerate(ends):
+        if end == 0:
+            continue
+        v = x[i, :end].double().view(end, G, C // G)
+        dims = (2,) if per_frame else (0, 2)
+        n = v.shape[2] * (1 if per_frame else end)
+        depth = 12 + 2 * math.sqrt(n)  # longest chain of additions of a blocked or pairwise sum
+        m = v.mean(dims, keepdim=True)
+        var = ((v - m) ** 2).mean(dims, keepdim=True)
+        r = 1 / torch.sqrt(var + eps)
+        em = depth * U * v.abs().mean(dims, keepdim=True)
+        # the mean's error moves every distance alike: var + em^2 instead of var
+        er = r * (U * (depth + 8) / 2 + 0.5 * em * em * r * r)
+        d = v - m
+        ed = em + U * (d.abs() + em)
+        nrm = (d * r).reshape(end, C)
+        en = (ed * r + d.abs() * er + 2 * U * (d * r).abs()).reshape(end, C)
+        z = nrm * wd + bd
+        ez = en * wd.abs() + 2 * U * ((nrm * wd).abs() + z.abs())
+        y[i, :end], e[i, :end] = _activate(z, ez, act)
+    return y, e
+
+
+NORM = [
+    # B, T, C, G, dtype, activation, per_frame, lengths
+    (1, 1, 8, 2, F32, None, False, None),
+    (1, 1, 64, 64, BF16, "silu", False, None),  # one value a group: the result is the bias
+    (2, 5, 80, 8, F32, "tanh", False, [5, 3]),
+    (3, 37, 80, 5, F16, "relu", False, [0, 37, 1]),
+    (3, 64, 512, 32, BF16, "silu", False, [64, 17, 50]),
+    (2, 861, 512, 32, BF16, "silu", False, None),
+    (1, 700, 1, 1, F32, None, False, None),
+    (2, 99, 7, 7, F32, "leaky_relu", False, [99, 98]),
+    (2, 333, 30, 3, BF16, "leaky_relu", False, [333, 200]),
+    (1, 4100, 256, 1, F16, None, False, None),  # one group as wide as the tensor
+    (2, 6000, 128, 16, F16, "leaky_relu", False, [5999, 4097]),
+    (1, 20001, 96, 6, F32, "silu", False, None),
+    (1, 3, 20000, 4, BF16, None, False, None),  # wide rows
+    (4, 3000, 33, 11, BF16, "tanh", False, [3000, 0, 2999, 1]),
+    (70000, 1, 4, 2, F32, None, False, None),  # more sequences than a 16-bit grid dimension holds
+    (64, 1, 1024, 8, BF16, "silu", True, None),
+    (3, 50, 80, 8, F32, "silu", True, [50, 0, 31]),
+    (2, 33, 1024, 1, F16, "tanh", True, None),
+    (2, 9, 5000, 2, BF16, None, True, [9, 4]),
+    (5, 21, 36, 12, F32, "relu", True, None),
+    (2, 17, 257, 1, BF16, "silu", True, None),
+    (1, 13, 64, 64, F32, None, True, None),
+    (2, 7, 12289, 1, F32, None, True, [7, 6]),
+]
+
+
+@pytest.mark.parametrize("B,T,C,G,dtype,act,per_frame,lengths", NORM)
+def test_group_norm(B, T, C, G, dtype, act, per_frame, lengths):
+    g = _rng(B * 7919 + T * 31 + C)
+    x = (torch.randn(B, T, C, generator=g) * (1 + torch.rand(C, generator=g)) + 0.5).to(dtype)
+    w, b = 1 + 0.2 * torch.randn(C, generator=g), 0.1 * torch.randn(C, generator=g)
+    ends = _ends(lengths, B, T)
+    for i, end in enumerate(ends):
+        x[i, end:] = float("nan")  # padding may hold anything
+    y = sequence.group_norm(x.cuda(), G, w.cuda(), b.cuda(), activation=act, per_frame=per_frame, lengths=_on(lengths))
+    assert y.dtype == dtype and y.is_contiguous()
+    _near(y, *norm_ref(x, G, w, b, 1e-5, act, per_frame, ends))
+    for i, end in enumerate(ends):
+        assert not y[i, end:].any()
+
+
+@pytest.mark.parametrize("T", [40, 3000, 30000])
+@pytest.mark.parametrize("offset", [1e3, -3e4])
+def test_group_norm_of_values_far_from_zero(T, offset):
+    """Spread 1 around a large mean: sums of squares would lose the variance (3e4^2 * 2^-24 > 50), distances do not."""
+    g = _rng(5)
+    x = torch.randn(2, T, 64, generator=g) + offset
+    y = sequence.group_norm(x.cuda(), 4)
+    _near(y, *norm_ref(x, 4, None, None, 1e-5, None, False, [T, T]))
+
+
+@pytest.mark.parametrize("dtype,C", [(F32, 64), (BF16, 64), (F16, 30), (F32, 7)])
+@pytest.mark.parametrize("per_frame", [False, True])
+@pytest.mark.parametrize("T", [45, 5000])
+def test_group_norm_strides_types_of_weights_and_missing_ones(dtype, C, per_frame, T):
+    g = _rng(3)
+    base = torch.randn(2, T, 2 * C + 1, generator=g).to(dtype)
+    G = 1 if C == 7 else 2
+    w, b = (1 + torch.randn(C, generator=g) * 0.1).to(dtype), torch.randn(C, generator=g).to(dtype)
+    dev = base.cuda()
+    lens = [T, T // 3]
+    views = [(base[..., C:2 * C], dev[..., C:2 * C]),  # rows 2C + 1 apart, starting anywhere
+             (base[..., 1:2 * C:2], dev[..., 1:2 * C:2]),  # channels not adjacent
+             (base[..., :C].transpose(0, 1).contiguous().transpose(0, 1),
+              dev[..., :C].transpose(0, 1).contiguous().transpose(0, 1)),  # [T][B][C] memory
+             (base[:1, :, :C].expand(2, T, C), dev[:1, :, :C].expand(2, T, C))]  # one sequence, used twice
+    for x, xd in views:
+        for wd, bd in ((w, b), (w, None), (None, b), (w.float(), b)):
+            y = sequence.group_norm(xd, G, wd if wd is None else wd.cuda(), bd if bd is None else bd.cuda(),
+                                    per_frame=per_frame, lengths=lens)
+            _near(y, *norm_ref(x, G, wd, bd, 1e-5, None, per_frame, lens))
+
+
+def test_group_norm_constant_and_non_finite_sequences():
+    x = torch.full((4, 50, 16), 3.25)
+    x[1, 20, 3] = float("inf")
+    x[2, 0, 9] = float("nan")
+    y = sequence.group_norm(x.cuda(), 2, bias=torch.full((16,), 0.5, device="cuda")).cpu()
+    assert (y[0] == 0.5).all() and (y[3] == 0.5).all()
+    assert y[1, :, :8].isnan().all() and (y[1, :, 8:] == 0.5).all()  # the group that holds it, and no other
+    assert (y[2, :, :8] == 0.5).all() and y[2, :, 8:].isnan().all()
+
+
+# --- causal convolution --------------------------------------------------------------------------------------------
+def conv_ref(x, w, b, act, state, ends):
+    """(y, error, state).  K products and sums: (K + 2) u of the sum of magnitudes."""
+    B, T, C = x.shape
+    K = w.size(1)
+    before = torch.zeros(B, K - 1, C, dtype=torch.float64) if state is None else state.double()
+    y, e, out = torch.zeros(B, T, C, dtype=torch.float64), torch.zeros(B, T, C, dtype=torch.float64), []
+    for i, end in enumerate(ends):
+        xp = torch.cat((before[i], x[i, :end].double()))
+        v = torch.zeros(end, C, dtype=torch.float64) if b is None else b.double().expand(end, C).clone()
+        a = v.abs()
+        for k in range(K):
+            v = v + w[:, k].double() * xp[k:k + end]
+            a = a + (w[:, k].double() * xp[k:k + end]).abs()
+        y[i, :end], e[i, :end] = _activate(v, (K + 2) * U * a, act)
+        out.append(xp[end:])
+    return y, e, torch.stack(out)
+
+
+CONV = [
+    # B, T, C, K, dtype, activation, state, lengths
+    (1, 1, 1, 1, F32, None, False, None),
+    (2, 1, 64, 4, BF16, "silu", True, None),
+    (512, 1, 1024, 4, BF16, "silu", True, None),
+    (3, 2, 40, 4, F32, "silu", True, [2, 0, 1]),  # fewer frames than taps: the state shifts
+    (3, 5, 40, 8, F16, "relu", True, [5, 3, 0]),
+    (2, 700, 1, 3, F32, None, True, None),
+    (2, 77, 33, 2, BF16, "tanh", True, [77, 50]),
+    (2, 77, 1023, 3, F32, None, False, None),
+    (3, 200, 1026, 4, BF16, "silu", True, [200, 199, 3]),
+    (2, 131, 136, 5, F16, "leaky_relu", True, None),
+    (2, 131, 100, 6, F32, "silu", True, [131, 64]),
+    (1, 1000, 24, 7, BF16, None, True, None),
+    (4, 861, 256, 4, BF16, "silu", True, [861, 1, 700, 0]),
+    (70000, 1, 2, 2, F32, None, True, None),
+]
+
+
+@pytest.mark.parametrize("B,T,C,K,dtype,act,state,lengths", CONV)
+def test_causal_conv(B, T, C, K, dtype, act, state, lengths):
+    g = _rng(B * 31 + T + C * 7 + K)
+    x = torch.randn(B, T, C, generator=g).to(dtype)
+    w, b = (torch.randn(C, K, generator=g) / math.sqrt(K)).to(dtype), (0.3 * torch.randn(C, generator=g)).to(dtype)
+    s = torch.randn(B, K - 1, C, generator=g).to(dtype) if state else None
+    ends = _ends(lengths, B, T)
+    for i, end in enumerate(ends):
+        x[i, end:] = float("nan")
+    out = torch.full((B, K - 1, C), 7.0, dtype=dtype, device="cuda")
+    y = sequence.causal_conv(x.cuda(), w.cuda(), b.cuda(), activation=act, state=None if s is None else s.cuda(),
+                             state_out=out, lengths=_on(lengths))
+    want, err, after = conv_ref(x, w, b, act, s, ends)
+    _near(y, want, err)
+    assert torch.equal(out.cpu().double(), after)  # inputs, copied
+    for i, end in enumerate(ends):
+        assert not y[i, end:].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("C", [64, 45])
+def test_causal_conv_strides_and_types_of_weights(dtype, C):
+    g = _rng(11)
+    T = 150
+    base = torch.randn(2, T, 2 * C + 3, generator=g).to(dtype)
+    dev = base.cuda()
+    w = (torch.randn(C, 1, 4, generator=g)).to(dtype)
+    lens = [T, 40]
+    for x, xd in ((base[..., 3:C + 3], dev[..., 3:C + 3]), (base[..., C:2 * C], dev[..., C:2 * C]),
+                  (base[..., :2 * C:2], dev[..., :2 * C:2]),
+                  (base[..., :C].transpose(0, 1).contiguous().transpose(0, 1),
+                   dev[..., :C].transpose(0, 1).contiguous().transpose(0, 1)),
+                  (base[:1, :, :C].expand(2, T, C), dev[:1, :, :C].expand(2, T, C))):
+        for wt in (w, w.float()):
+            y = sequence.causal_conv(xd, wt.cuda(), lengths=lens)
+            _near(y, *conv_ref(x, wt[:, 0], None, None, None, lens)[:2])
+
+
+def test_causal_conv_relu_takes_minus_infinity_to_zero_and_keeps_a_nan():
+    x = torch.tensor([[1.0, float("-inf"), 2.0, float("nan"), 3.0]]).view(1, 5, 1).cuda()
+    y = sequence.causal_conv(x, torch.ones(1, 1, device="cuda"), activation="relu").cpu().view(-1)
+    assert y[0] == 1 and y[1] == 0 and y[2] == 2 and y[3].isnan() and y[4] == 3
+
+
+# --- selective scan ------------------------------------------------------------------------------------------------
+def scan_ref(u, delta, A, Bm, Cm, D, z, bias, softplus, state, ends):
+    """(y, error of y, h, error of h).
+
+    Per frame: dt is off by 10 u of itself (bias, exp2, reciprocal, series, and |v| u from exp2's argument);
+    its error moves the decay a = exp(dt A) by |dt A| times that, exp2's argument adds 2 |dt A| u and the function 2 u; dt *
+    u * B adds 3 roundings.  Running: E <- a E + a |h| u (4 + 14 |dt A|) + |dt u B| u 14 + |h| u.  A scan cut into pieces
+    sums dt over a piece and applies one decay exp(A S) to the state before it: S of up to 256 frames is off by under 24 u of
+    itself in a blocked sum, or its length in a serial one, and |A S| exp(A S) <= 0.37: 256 * 0.37 u of |h| at most, once."""
+    Bn, T, Dn = u.shape
+    N = A.size(1)
+    G = Bm.size(2)
+    h = torch.zeros(Bn, Dn, N, dtype=torch.float64) if state is None else state.double().clone()
+    mag, E = h.abs(), torch.zeros_like(h)
+    y, ey = torch.zeros(Bn, T, Dn, dtype=torch.float64), torch.zeros(Bn, T, Dn, dtype=torch.float64)
+    v = delta.double() + (0 if bias is None else bias.double())
+    dt = torch.nn.functional.softplus(v) if softplus else v
+    edt = (10 + 2 * v.abs()) * U * dt.abs() + U * (v - delta.double()).abs()
+    grp = torch.arange(Dn) // (Dn // G)
+    Ad = A.double()
+    live = torch.tensor(ends)[:, None] > torch.arange(T)[None]
+    clean = lambda t, t_i: torch.where(live[:, t_i].view(-1, *([1] * (t.dim() - 1))), t, torch.zeros_like(t))  # noqa: E731
+    for t in range(T):
+        d, ed, ut = clean(dt[:, t], t)[..., None], clean(edt[:, t], t)[..., None], clean(u[:, t].double(), t)
+        b, c = clean(Bm[:, t].double(), t)[:, grp], clean(Cm[:, t].double(), t)[:, grp]
+        a = torch.exp(d * Ad)
+        x = d * ut[..., None] * b
+        k = live[:, t].view(-1, 1, 1)
+        E = torch.where(k, a * E + a * mag * ((4 + 4 * (d * Ad).abs()) * U + ed * Ad.abs())
+                        + x.abs() * 4 * U + (ed * ut[..., None] * b).abs() + U * (a * mag + x.abs()), E)
+        h = torch.where(k, a * h + x, h)
+        mag = torch.where(k, a * mag + x.abs(), mag)
+        S = (N + 3) * U
+        o, eo = (h * c).sum(-1), (E * c.abs() + 100 * U * mag * c.abs()).sum(-1) + S * (mag * c.abs()).sum(-1)
+        if D is not None:
+            o, eo = o + D.double() * ut, eo + 2 * U * (D.double() * ut).abs() + U * o.abs()
+        if z is not None:
+            zt = clean(z[:, t].double(), t)
+            gt = zt * torch.sigmoid(zt)
+            eo = eo * gt.abs() + o.abs() * gt.abs() * U * (9 + 2 * zt.abs())
+            o = o * gt
+        y[:, t], ey[:, t] = clean(o, t), clean(eo, t)
+    return y, ey, h, E + 100 * U * mag
+
+
+def scan_inputs(B, T, D, N, G, dtype, gate, state, seed, bias=True):
+    g = _rng(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    step = torch.exp(torch.rand(D, generator=g) * math.log(100.0) + math.log(0.001))
+    return dict(u=r(B, T, D).to(dtype), delta=(0.5 * r(B, T, D)).to(dtype),
+                A=-torch.arange(1, N + 1).float() * torch.exp(0.2 * r(D, N)), Bm=r(B, T, G, N).to(dtype),
+                Cm=r(B, T, G, N).to(dtype), D=1 + 0.1 * r(D), z=r(B, T, D).to(dtype) if gate else None,
+                bias=step + torch.log(-torch.expm1(-step)) if bias else None, state=r(B, D, N) if state else None)
+
+
+def scan_run(p, softplus, lengths, state_out=None, **over):
+    q = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in {**p, **over}.items()}
+    return sequence.selective_scan(q["u"], q["delta"], q["A"], q["Bm"], q["Cm"], D=q["D"], z=q["z"], delta_bias=q["bias"],
+                                   delta_softplus=softplus, state=q["state"], state_out=state_out, lengths=lengths)
+
+
+SCAN = [
+    # B, T, D, N, G, dtype, gate, state, lengths
+    (1, 1, 1, 1, 1, F32, False, False, None),
+    (1, 1, 1024, 16, 1, BF16, True, True, None),
+    (96, 1, 80, 16, 1, F16, True, True, None),
+    (5, 1, 250, 12, 2, F32, False, True, [1, 0, 1, 1, 0]),
+    (3, 2, 64, 16, 1, BF16, True, True, [2, 0, 1]),
+    (2, 5, 48, 8, 3, F32, True, True, [5, 4]),
+    (2, 64, 64, 16, 1, BF16, True, False, None),
+    (3, 129, 100, 16, 2, F32, True, True, [129, 0, 65]),
+    (2, 333, 250, 12, 2, F32, False, True, None),
+    (1, 1500, 32, 16, 1, F16, True, True, None),
+    (4, 600, 64, 16, 1, BF16, True, True, [600, 1, 599, 0]),
+    (1, 2500, 17, 5, 1, F32, False, True, None),
+    (2, 300, 30, 64, 3, F32, True, True, [300, 191]),
+    (1, 400, 64, 33, 1, BF16, False, True, None),
+    (1, 400, 64, 1, 4, F32, False, True, None),
+    (1, 500, 24, 4, 24, F16, True, True, None),  # a group to each channel
+    (2, 257, 640, 16, 4, BF16, True, True, [257, 256]),
+    (40, 70, 512, 16, 1, BF16, True, False, None),
+    (70000, 1, 2, 2, 1, F32, False, True, None),
+]
+
+
+@pytest.mark.parametrize("B,T,D,N,G,dtype,gate,state,lengths", SCAN)
+def test_selective_scan(B, T, D, N, G, dtype, gate, state, lengths):
+    p = scan_inputs(B, T, D, N, G, dtype, gate, state, B + 17 * T + D + N)
+    ends = _ends(lengths, B, T)
+    for i, end in enumerate(ends):
+        for k in ("u", "delta", "Bm", "Cm", "z"):
+            if p[k] is not None:
+                p[k][i, end:] = float("nan")
+    out = torch.full((B, D, N), 7.0, device="cuda")
+    y = scan_run(p, True, _on(lengths), out)
+    want, err, h, eh = scan_ref(softplus=True, ends=ends, **p)
+    _near(y, want, err, "y")
+    _near(out, h, eh, "state")
+    for i, end in enumerate(ends):
+        assert not y[i, end:].any()
+
+
+@pytest.mark.parametrize("T", [1, 700])
+def test_selective_scan_without_softplus_bias_and_skip(T):
+    p = scan_inputs(2, T, 40, 8, 1, F32, False, False, 4, bias=False)
+    p["delta"], p["D"] = p["delta"].abs() * 0.1, None
+    y = scan_run(p, False, None)
+    want, err, _, _ = scan_ref(softplus=False, ends=[T, T], **p)
+    _near(y, want, err)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 90, 1100])
+def test_selective_scan_takes_slices_of_projections(dtype, T):
+    B, D, N, G, R = 2, 66, 10, 2, 7
+    g = _rng(9)
+    p = scan_inputs(B, T, D, N, G, dtype, True, True, 6)
+    xz = torch.randn(B, T, 2 * D + 1, generator=g).to(dtype)
+    dbc = torch.randn(B, T, R + 2 * G * N, generator=g).to(dtype)
+    xzd, dbcd = xz.cuda(), dbc.cuda()
+    view = lambda a, b: dict(u=a[..., 1:D + 1], z=a[..., D + 1:], Bm=b[..., R:R + G * N].unflatten(-1, (G, N)),  # noqa: E731
+                             Cm=b[..., R + G * N:].unflatten(-1, (G, N)))
+    want, err, h, eh = scan_ref(softplus=True, ends=[T, T // 2], **{**p, **view(xz, dbc)})
+    out = torch.empty(B, D, N, device="cuda")
+    y = scan_run(p, True, [T, T // 2], out, **view(xzd, dbcd))
+    _near(y, want, err)
+    _near(out, h, eh)
+    # the same from [T][B] memory, with channels that are not adjacent, and with bfloat16 parameters widened first
+    tb = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    y2 = scan_run(p, True, [T, T // 2], out, **{k: tb(v) for k, v in view(xzd, dbcd).items()})
+    assert torch.equal(y2, y)
+    wide = p["delta"].cuda().repeat_interleave(2, -1)[..., ::2]
+    y3 = scan_run(p, True, [T, T // 2], out, **{**view(xzd, dbcd), "delta": wide})
+    assert torch.equal(y3, y)
+
+
+@pytest.mark.parametrize("T", [3, 1000])
+def test_selective_scan_extreme_steps(T):
+    """Steps that underflow (softplus of -80), steps that forget everything (dt A far below -126 in base 2) and a state that
+    is never touched: no NaN comes of 0 * inf or inf - inf, and small steps keep their relative precision."""
+    p = scan_inputs(1, T, 64, 16, 1, F32, False, True, 2)
+    p["delta"][..., :16] = -80.0
+    p["delta"][..., 16:32] = 200.0
+    p["delta"][..., 32:48] = -17.0  # softplus = 4e-8
+    p["bias"] = None
+    out = torch.empty(1, 64, 16, device="cuda")
+    y = scan_run(p, True, None, out)
+    want, err, h, eh = scan_ref(softplus=True, ends=[T], **p)
+    assert torch.isfinite(y).all() and torch.isfinite(out).all()
+    _near(y, want, err)
+    _near(out, h, eh)
+
+
+# --- carried states ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cuts", [[1] * 9, [1, 1, 7], [4, 5], [300, 1, 1, 2, 500]])
+def test_a_sequence_cut_into_calls_equals_one_call(dtype, cuts):
+    """States replaced in place; the convolution copies, so it is equal bit for bit, the scan is held to its reference."""
+    T, B, D, N = sum(cuts), 2, 48, 16
+    p = scan_inputs(B, T, D, N, 1, dtype, True, True, 21)
+    w = torch.randn(D, 4, generator=_rng(1)).to(dtype).cuda()
+    u = p["u"].cuda()
+    whole = sequence.causal_conv(u, w, activation="silu")
+    cs, hs = torch.zeros(B, 3, D, dtype=dtype, device="cuda"), p["state"].cuda()
+    conv, scan, at = [], [], 0
+    for n in cuts:
+        part = slice(at, at + n)
+        conv.append(sequence.causal_conv(u[:, part], w, activation="silu", state=cs, state_out=cs))
+        q = {k: p[k][:, part] for k in ("u", "delta", "Bm", "Cm", "z")}
+        scan.append(scan_run(p, True, None, hs, **q, state=hs))
+        at += n
+    assert torch.equal(torch.cat(conv, 1), whole)
+    want, err, h, eh = scan_ref(softplus=True, ends=[T] * B, **p)
+    _near(torch.cat(scan, 1), want, 4 * err)  # (cut differently from the reference's one piece: its bound, per piece)
+    _near(hs, h, 4 * eh)
+
+
+@pytest.mark.parametrize("T", [1, 4, 700])
+def test_state_in_place_equals_state_elsewhere_and_no_frames_leave_it(T):
+    p = scan_inputs(3, T, 80, 16, 1, BF16, True, True, 8)
+    lens = [T, 0, max(1, T // 2)]
+    out, place = torch.empty(3, 80, 16, device="cuda"), p["state"].cuda()
+    y1 = scan_run(p, True, lens, out)
+    y2 = scan_run(p, True, lens, place, state=place)
+    assert torch.equal(y1, y2) and torch.equal(out, place) and torch.equal(place[1].cpu(), p["state"][1])
+    x, w = p["u"].cuda(), torch.randn(80, 4, generator=_rng(2)).cuda()
+    s = torch.randn(3, 3, 80, generator=_rng(3)).to(BF16).cuda()
+    c_out, c_place = torch.empty_like(s), s.clone()
+    y1 = sequence.causal_conv(x, w, state=s, state_out=c_out, lengths=lens)
+    y2 = sequence.causal_conv(x, w, state=c_place, state_out=c_place, lengths=lens)
+    assert torch.equal(y1, y2) and torch.equal(c_out, c_place) and torch.equal(c_place[1], s[1])
+
+
+def test_calls_without_frames_or_sequences():
+    h, s = torch.randn(2, 8, 4, device="cuda"), torch.randn(2, 3, 8, device="cuda")
+    ho, so = torch.zeros_like(h), torch.zeros_like(s)
+    e = lambda *n: torch.empty(*n, device="cuda")  # noqa: E731
+    A, w = -torch.ones(8, 4, device="cuda"), torch.ones(8, 4, device="cuda")
+    y = sequence.selective_scan(e(2, 0, 8), e(2, 0, 8), A, e(2, 0, 4), e(2, 0, 4), state=h, state_out=ho)
+    assert y.shape == (2, 0, 8) and torch.equal(ho, h)
+    y = sequence.causal_conv(e(2, 0, 8), w, state=s, state_out=so)
+    assert y.shape == (2, 0, 8) and torch.equal(so, s)
+    sequence.selective_scan(e(2, 0, 8), e(2, 0, 8), A, e(2, 0, 4), e(2, 0, 4), state_out=ho)
+    sequence.causal_conv(e(2, 0, 8), w, state_out=so)
+    assert not ho.any() and not so.any()
+    assert sequence.group_norm(e(2, 0, 8), 2).shape == (2, 0, 8) and sequence.group_norm(e(0, 3, 8), 2).shape == (0, 3, 8)
+    assert sequence.causal_conv(e(0, 5, 8), w).shape == (0, 5, 8)
+    assert sequence.selective_scan(e(0, 8), e(0, 8), A, e(0, 4), e(0, 4)).shape == (0, 8)
+
+
+# --- as they are used ----------------------------------------------------------------------------------------------
+class _Block:
+    """norm -> projection -> convolution -> projections -> scan -> projection, added to its input."""
+
+    def __init__(self, dim, inner, N, dtype, seed):
+        g = _rng(seed)
+        r = lambda *s, k=1.0: (k * torch.randn(*s, generator=g)).to(dtype).cuda()  # noqa: E731
+        self.R, self.N, self.inner = max(1, inner // 16), N, inner
+        self.g, self.b = 1 + 0.1 * torch.randn(dim, generator=g).cuda(), 0.1 * torch.randn(dim, generator=g).cuda()
+        self.w_in, self.w_x = r(2 * inner, dim, k=dim ** -0.5), r(self.R + 2 * N, inner, k=inner ** -0.5)
+        self.w_dt, self.w_out = r(inner, self.R, k=self.R ** -0.5), r(dim, inner, k=inner ** -0.5)
+        self.taps, self.tap_bias = r(inner, 4, k=0.5), r(inner, k=0.1)
+        self.A = (-torch.arange(1, N + 1).float() * torch.exp(0.1 * torch.randn(inner, N, generator=g))).cuda()
+        self.D, self.dt_bias = torch.ones(inner, device="cuda"), torch.full((inner,), -3.0, device="cuda")
+
+    def states(self, B, dtype):
+        return (torch.zeros(B, 3, self.inner, dtype=dtype, device="cuda"), torch.zeros(B, self.inner, self.N, device="cuda"))
+
+    def __call__(self, x, states, lengths=None):
+        conv, h = states
+        y = sequence.group_norm(x, 8, self.g, self.b, activation="silu", per_frame=True, lengths=lengths)
+        u, z = (y @ self.w_in.T).chunk(2, -1)
+        u = sequence.causal_conv(u, self.taps, self.tap_bias, activation="silu", state=conv, state_out=conv, lengths=lengths)
+        low, B, C = (u @ self.w_x.T).split((self.R, self.N, self.N), -1)
+        y = sequence.selective_scan(u, low @ self.w_dt.T, self.A, B, C, D=self.D, z=z, delta_bias=self.dt_bias,
+                                    delta_softplus=True, state=h, state_out=h, lengths=lengths)
+        return x + y @ self.w_out.T
+
+
+@torch.no_grad()
+def test_prompt_then_captured_single_frames_equal_the_whole_sequence():
+    """A stack of two blocks: ragged prompts in one padded call, then frame by frame from a captured graph, replayed with
+    eager work between the replays, against the same frames in one float32 call of each sequence by itself."""
+    B, T, steps, dim = 3, 41, 6, 64
+    stack = [_Block(dim, 128, 16, F32, 40 + i) for i in range(2)]
+    x = torch.randn(B, T + steps, dim, generator=_rng(7)).cuda()
+    lens = [41, 17, 2]
+
+    def run(v, st, lengths=None):
+        for blk, s in zip(stack, st):
+            v = blk(v, s, lengths)
+        return v
+
+    whole = []
+    for b, n in enumerate(lens):
+        one = torch.cat((x[b:b + 1, :n], x[b:b + 1, T:]), 1)
+        whole.append(run(one, [blk.states(1, F32) for blk in stack])[0])
+    st = [blk.states(B, F32) for blk in stack]
+    padded = x[:, :T].clone()
+    for b, n in enumerate(lens):
+        padded[b, n:] = 1e4  # padding holds whatever was there
+    prompt = run(padded, st, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    # float32 products in another order, through two blocks: a few hundred roundings at most
+    close = dict(rtol=0, atol=1000 * U * float(torch.cat(whole).abs().max()))
+    for b, n in enumerate(lens):
+        assert torch.allclose(prompt[b, :n], whole[b][:n], **close)
+    frame = x[:, T].clone()
+    kept = [[s.clone() for s in p] for p in st]
+    run(frame, [[s.clone() for s in p] for p in st])  # (libraries and allocator warm before the capture)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(frame, st)
+    for p, k in zip(st, kept):
+        for s, c in zip(p, k):
+            s.copy_(c)
+    for t in range(steps):
+        frame.copy_(x[:, T + t])
+        eager = run(x[:, T + t], [[s.clone() for s in p] for p in st])  # the program's own work between replays
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        for b, n in enumerate(lens):
+            assert torch.allclose(out[b], whole[b][n + t], **close), (b, t)
+
+
+@torch.no_grad()
+def test_two_captured_prompts_replayed_side_by_side_do_not_share_scratch():
+    """Long calls that use scratch memory, captured one after the other on one stream and replayed at once on two."""
+    ps = [scan_inputs(1, 3000, 64, 16, 1, BF16, True, False, 50 + i) for i in range(2)]
+    xs = [torch.randn(1, 30000, 64, generator=_rng(60 + i)).cuda() for i in range(2)]
+    qs = [{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in p.items()} for p in ps]
+    work = lambda i: (scan_run(qs[i], True, None), sequence.group_norm(xs[i], 4))  # noqa: E731
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(i))
+        graphs.append(g)
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(side[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+
+
+@torch.no_grad()
+def test_results_do_not_depend_on_the_run_or_the_stream():
+    p = scan_inputs(2, 2000, 96, 16, 1, F32, True, True, 70)
+    x = torch.randn(2, 9000, 96, generator=_rng(71)).cuda()
+    lens = torch.tensor([2000, 1234], dtype=torch.int32, device="cuda")
+    work = lambda: (scan_run(p, True, lens), sequence.group_norm(x, 6, activation="silu"),  # noqa: E731
+                    sequence.causal_conv(x, torch.ones(96, 4, device="cuda")))
+    first = work()
+    side = torch.cuda.Stream()
+    for i in range(4):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            again = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+# --- the C entry points on their own -------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 50, 5000])
+def test_only_the_outputs_are_written(T):
+    """Guard bands around every output, rows of the outputs further apart than their channels, lengths out of range."""
+    import ctypes
+
+    B, C, N, K, pad = 2, 40, 16, 4, 24
+    dev = torch.device("cuda")
+    x = torch.randn(B, T, C, generator=_rng(80)).to(BF16).cuda()
+    bc = torch.randn(B, T, 1, N, generator=_rng(81)).to(BF16).cuda()
+    w, A = torch.ones(C, K, device=dev), -torch.ones(C, N, device=dev)
+    row = C + pad
+    lens = torch.tensor([T + 9, -3], dtype=torch.int32, device=dev)
+    lib, st = _native.lib(), torch.cuda.current_stream().cuda_stream
+    at = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
+    for op in ("norm", "frame", "conv", "scan"):
+        big = torch.full((B * T * row + 2 * row,), 7.0, dtype=BF16, device=dev)
+        y = (big.data_ptr() + 2 * row, T * row, row)
+        s = torch.full((64 + B * C * N + 64,), 7.0, device=dev)
+        ws = torch.full((1 << 22,), 90, dtype=torch.uint8, device=dev)
+        if op in ("norm", "frame"):
+            a = _native.mv_group_norm_args(*at(x), *y, None, None, lens.data_ptr(), B, T, C, 4, 1, 0, int(op == "frame"), 1,
+                                           0.1, 1e-5)
+            n = lib.mv_group_norm_workspace(ctypes.byref(a))
+            rc = lib.mv_group_norm(ctypes.byref(a), ws.data_ptr() + 4096, n, st)
+            want = sequence.group_norm(x, 4, activation="silu", per_frame=op == "frame", lengths=lens)
+            if n:
+                assert lib.mv_group_norm(ctypes.byref(a), ws.data_ptr() + 4096, n - 1, st) == -4
+        elif op == "conv":
+            n = 0
+            sb = torch.full((64 + B * (K - 1) * C + 64,), 7.0, dtype=BF16, device=dev)
+            a = _native.mv_causal_conv_args(*at(x), *y, w.data_ptr(), None, None, sb.data_ptr() + 128, lens.data_ptr(), B, T,
+                                            C, K, 1, 0, 0, 0.1)
+            rc = lib.mv_causal_conv(ctypes.byref(a), st)
+            want = sequence.causal_conv(x, w, lengths=lens)
+            assert (sb[:64] == 7).all() and (sb[-64:] == 7).all() and not sb[64 + (K - 1) * C:-64].any()
+        else:
+            a = _native.mv_selective_scan_args(*at(x), *at(x), None, 0, 0, *at(bc), *at(bc), 0, 0, *y, A.data_ptr(), None, None,
+                                               None, s.data_ptr() + 256, lens.data_ptr(), B, T, C, N, 1, 1, 1)
+            n = lib.mv_selective_scan_workspace(ctypes.byref(a))
+            rc = lib.mv_selective_scan(ctypes.byref(a), ws.data_ptr() + 4096, n, st)
+            want = sequence.selective_scan(x, x, A, bc, bc, delta_softplus=True, lengths=lens)
+            assert (s[:64] == 7).all() and (s[-64:] == 7).all() and not s[64 + C * N:-64].any()
+            if n:
+                assert lib.mv_selective_scan(ctypes.byref(a), ws.data_ptr() + 4096, n - 1, st) == -4
+        assert rc == 0, lib.mv_last_error()
+        torch.cuda.synchronize()
+        assert 4096 + n < ws.numel() - 4096 and (ws[:4096] == 90).all() and (ws[4096 + n:] == 90).all()
+        got = big[row:-row].view(B, T, row)
+        assert (big[:row] == 7).all() and (big[-row:] == 7).all() and (got[..., C:] == 7).all()
+        assert torch.equal(got[..., :C], want) and not got[1, :, :C].any()
+
+
+def test_group_norm_in_place():
+    for T in (30, 6000):
+        x = torch.randn(2, T, 64, generator=_rng(90)).cuda()
+        want = sequence.group_norm(x, 4, activation="tanh")
+        import ctypes
+
+        a = _native.mv_group_norm_args(x.data_ptr(), T * 64, 64, x.data_ptr(), T * 64, 64, None, None, None, 2, T, 64, 4, 0, 0,
+                                       0, 3, 0.1, 1e-5)
+        lib = _native.lib()
+        n = lib.mv_group_norm_workspace(ctypes.byref(a))
+        ws = torch.empty(n + 256, dtype=torch.uint8, device="cuda")
+        assert lib.mv_group_norm(ctypes.byref(a), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+
+
+# --- refusals ------------------------------------------------------------------------------------------------------
+def test_refusals():
+    f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    x, w, A, bc = f(2, 5, 8), f(8, 4), f(8, 4), f(2, 5, 4)
+    norm, conv, scan = sequence.group_norm, sequence.causal_conv, sequence.selective_scan
+    bad = [
+        lambda: norm(x, 3), lambda: norm(x, 0), lambda: norm(x, 2, eps=-1.0), lambda: norm(f(8), 2),
+        lambda: norm(x.double(), 2), lambda: norm(x, 2, weight=f(7)), lambda: norm(x, 2, weight=f(8).half()),
+        lambda: norm(x, 2, weight=torch.zeros(8)), lambda: norm(x, 2, lengths=[5]), lambda: norm(x, 2, lengths=[5, 6]),
+        lambda: norm(x, 2, lengths=[-1, 5]), lambda: norm(x, 2, lengths=torch.ones(2, device="cuda")),
+        lambda: conv(x, f(7, 4)), lambda: conv(x, f(8, 9)), lambda: conv(x, f(8, 0)), lambda: conv(x, f(8, 2, 4)),
+        lambda: conv(x, w, state=f(2, 4, 8)), lambda: conv(x, w, state_out=f(1, 3, 8)),
+        lambda: conv(x, w, state=f(2, 3, 8).half()), lambda: conv(x, w, state=f(1, 3, 8).expand(2, 3, 8)),
+        lambda: conv(x, w, state=f(2, 8, 3).transpose(1, 2)), lambda: conv(x.half(), w.bfloat16()),
+        lambda: scan(x, f(2, 5, 7), A, bc, bc), lambda: scan(x, x.half(), A, bc, bc), lambda: scan(x, x, f(7, 4), bc, bc),
+        lambda: scan(x, x, f(8, 65), f(2, 5, 65), f(2, 5, 65)), lambda: scan(x, x, A, f(2, 5, 5), bc),
+        lambda: scan(x, x, A, bc, f(2, 4, 4)), lambda: scan(x, x, A, f(2, 5, 3, 4), f(2, 5, 3, 4)),
+        lambda: scan(x, x, A, f(2, 5, 2, 4), bc), lambda: scan(x, x, A, bc, bc, D=f(4)), lambda: scan(x, x, A, bc.half(), bc),
+        lambda: scan(x, x, A, bc, bc, z=f(2, 5, 4)), lambda: scan(x, x, A, bc, bc, state=f(2, 8, 4).half()),
+        lambda: scan(x, x, A.double(), bc, bc), lambda: scan(x, x, A, bc, bc, state_out=f(8, 2, 4).transpose(0, 1)),
+        lambda: scan(f(2, 8), f(2, 8), A, bc, bc), lambda: scan(x, x, A, torch.zeros(2, 5, 4), bc),
+        lambda: norm(x.clone().requires_grad_(), 2), lambda: conv(x, w.clone().requires_grad_()),
+        lambda: scan(x, x, A.clone().requires_grad_(), bc, bc),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    for call in (lambda: norm(x, 2, activation="gelu"), lambda: conv(x, w, activation="none")):
+        with pytest.raises(ValueError):
+            call()
+    h = f(3, 8, 4)
+    with pytest.raises(_native.MelvocError, match="overlap"):
+        scan(x, x, A, bc, bc, state=h[:2], state_out=h[1:])
+    with torch.no_grad():  # a model's parameters, at synthesis
+        norm(x, 2, weight=f(8).requires_grad_())
+    # counts that do not fit 32 bits are clamped like any other
+    long = torch.tensor([2 ** 32 + 1, -2 ** 40], device="cuda")
+    assert torch.equal(norm(torch.ones(2, 5, 8, device="cuda"), 2, bias=torch.ones(8, device="cuda"), lengths=long)[:, :, 0],
+                       torch.tensor([[1.0] * 5, [0.0] * 5], device="cuda"))

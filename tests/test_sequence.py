@@ -1,0 +1,84 @@
+"""The sequence operators' C entry points refuse what they cannot compute before anything reaches a device: every call here
+carries made-up pointers and must come back with an error code and a message."""
+import ctypes
+import os
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tacotron2_amd import _native, sequence  # noqa: E402
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_native.LIB_PATH), reason="libmelvoc.so is not built")
+P = 1 << 20  # a made-up, well aligned device address
+
+
+def _norm(**k):
+    a = _native.mv_group_norm_args(P, 320, 32, 2 * P, 320, 32, P, P, None, 2, 10, 32, 4, 0, 0, 0, 1, 0.1, 1e-5)
+    for f, v in k.items():
+        setattr(a, f, v)
+    return _native.lib().mv_group_norm(ctypes.byref(a), None, 0, None)
+
+
+def _conv(**k):
+    a = _native.mv_causal_conv_args(P, 320, 32, 2 * P, 320, 32, P, P, 3 * P, 3 * P, None, 2, 10, 32, 4, 0, 0, 1, 0.1)
+    for f, v in k.items():
+        setattr(a, f, v)
+    return _native.lib().mv_causal_conv(ctypes.byref(a), None)
+
+
+def _scan(**k):
+    a = _native.mv_selective_scan_args(P, 320, 32, P, 320, 32, None, 0, 0, P, 160, 16, P, 160, 16, 0, 0, 2 * P, 320, 32, P, P,
+                                       P, 3 * P, 3 * P, None, 2, 10, 32, 16, 1, 0, 1)
+    for f, v in k.items():
+        setattr(a, f, v)
+    return _native.lib().mv_selective_scan(ctypes.byref(a), None, 0, None)
+
+
+BAD = [
+    (_norm, dict(groups=0), b"groups"), (_norm, dict(groups=5), b"groups"), (_norm, dict(B=-1), b"sizes"),
+    (_norm, dict(T=-1), b"sizes"), (_norm, dict(C=0), b"sizes"), (_norm, dict(dtype=3), b"dtype"),
+    (_norm, dict(weight_dtype=1), b"weight_dtype"), (_norm, dict(activation=4), b"activation"),
+    (_norm, dict(eps=-1e-5), b"eps"), (_norm, dict(eps=float("nan")), b"eps"), (_norm, dict(eps=float("inf")), b"eps"),
+    (_norm, dict(x=None), b"x needs"), (_norm, dict(y=None), b"output needs"), (_norm, dict(x=P + 2), b"x needs"),
+    (_norm, dict(x_row_stride=-32), b"strides"), (_norm, dict(y_row_stride=31), b"overlap"),
+    (_norm, dict(y_batch_stride=319), b"overlap"), (_norm, dict(y_batch_stride=31, y_row_stride=64), b"overlap"),
+    (_conv, dict(K=0), b"taps"), (_conv, dict(K=9), b"taps"), (_conv, dict(weight=None), b"weight"),
+    (_conv, dict(weight_dtype=2), b"weight"), (_conv, dict(activation=-1), b"activation"), (_conv, dict(dtype=-1), b"dtype"),
+    (_conv, dict(state_out=3 * P + 64), b"overlap"), (_conv, dict(state_out=3 * P - 64), b"overlap"),
+    (_conv, dict(x=None), b"x needs"), (_conv, dict(y=P + 1), b"output needs"), (_conv, dict(y_row_stride=16), b"overlap"),
+    (_scan, dict(N=0), b"states"), (_scan, dict(N=65), b"states"), (_scan, dict(G=0), b"groups"), (_scan, dict(G=3), b"groups"),
+    (_scan, dict(A=None), b"needs A"), (_scan, dict(u=None), b"u needs"), (_scan, dict(delta=None), b"delta needs"),
+    (_scan, dict(Bm=None), b"Bm needs"), (_scan, dict(Cm=None), b"Cm needs"), (_scan, dict(z=P + 2), b"z needs"),
+    (_scan, dict(y=None), b"output needs"), (_scan, dict(y_batch_stride=0), b"overlap"),
+    (_scan, dict(state_out=3 * P + 4), b"overlap"), (_scan, dict(dtype=7), b"dtype"), (_scan, dict(D=0), b"sizes"),
+    (_scan, dict(B=-2), b"sizes"),
+]
+
+
+@pytest.mark.parametrize("call,fields,message", BAD, ids=lambda v: v if isinstance(v, str) else None)
+def test_bad_arguments_are_refused_before_a_launch(call, fields, message):
+    assert call(**fields) == -1
+    assert message in _native.lib().mv_last_error(), _native.lib().mv_last_error()
+
+
+def test_null_arguments_and_empty_calls():
+    lib = _native.lib()
+    assert lib.mv_group_norm(None, None, 0, None) == -1
+    assert lib.mv_causal_conv(None, None) == -1
+    assert lib.mv_selective_scan(None, None, 0, None) == -1
+    assert lib.mv_group_norm_workspace(None) == 0 and lib.mv_selective_scan_workspace(None) == 0
+    # nothing to do: no pointer is looked at, nothing is launched
+    assert _norm(B=0, x=None, y=None) == 0 and _norm(T=0, x=None, y=None) == 0
+    assert _conv(B=0, x=None, y=None) == 0 and _conv(T=0, x=None, y=None) == 0  # (the state stays where it is)
+    assert _scan(B=0, u=None, A=None, y=None) == 0 and _scan(T=0, u=None, y=None) == 0
+
+
+def test_there_is_no_cpu_path():
+    x = torch.zeros(2, 5, 8)
+    with pytest.raises(RuntimeError, match="MI355X only"):
+        sequence.group_norm(x, 2)
+    with pytest.raises(RuntimeError, match="MI355X only"):
+        sequence.causal_conv(x, torch.zeros(8, 4))
+    with pytest.raises(RuntimeError, match="MI355X only"):
+        sequence.selective_scan(x, x, torch.zeros(8, 4), torch.zeros(2, 5, 4), torch.zeros(2, 5, 4))
