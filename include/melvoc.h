@@ -226,7 +226,7 @@ MV_API int mv_pcm16(const float* wav, size_t n, int16_t* pcm, void* stream);
  * convolution and the selective state space scan, the last two for prompts and for single frames (state in, state out).
  *
  * A tensor is [B][T][C] with adjacent channels and any batch and row stride (mv_rows; strides in elements, so halves of a
- * projection's output or [T][B][C] memory are taken as they lie).  Data are float32, bfloat16 or float16 (`dtype`),
+ * projection's output or [T][B][C] memory are taken as they lie; row strides up to 2^25).  Data are float32, bfloat16 or float16 (`dtype`),
  * arithmetic is float32 with one rounding at the store; float16 results beyond its range become infinities.  `lengths` is a
  * device int32 [B] of true frame counts or NULL (all T); entries are clamped into [0, T] by the kernels.  Frames at or past
  * a sequence's end are never read into a result and are written as 0.  Calls run on the current HIP device, are
@@ -263,7 +263,7 @@ typedef struct mv_group_norm_args {
     float slope;        /* of MV_ACT_LRELU */
     float eps;          /* >= 0 */
 } mv_group_norm_args;
-/* scratch of mv_group_norm in bytes (256-byte aligned; 0: none needed, workspace may be NULL) */
+/* scratch of mv_group_norm in bytes (256-byte aligned; 0: none needed, workspace may be NULL; T = 1 never needs any) */
 MV_API size_t mv_group_norm_workspace(const mv_group_norm_args* a);
 MV_API int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -307,7 +307,7 @@ typedef struct mv_selective_scan_args {
     int dtype;               /* MV_DTYPE_* of u, delta, z, Bm, Cm and y */
     int delta_softplus;
 } mv_selective_scan_args;
-/* scratch of mv_selective_scan in bytes (256-byte aligned; 0: none needed, workspace may be NULL) */
+/* scratch of mv_selective_scan in bytes (256-byte aligned; 0: none needed, workspace may be NULL; T = 1 never needs any) */
 MV_API size_t mv_selective_scan_workspace(const mv_selective_scan_args* a);
 MV_API int mv_selective_scan(const mv_selective_scan_args* a, void* workspace, size_t workspace_bytes, void* stream);
 

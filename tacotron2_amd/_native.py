@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -100,6 +101,14 @@ class mv_selective_scan_args(C.Structure):
                 + _fields(C.c_int, "B T D N G dtype delta_softplus"))
 
 
+def _packer(args):
+    """struct.Struct that packs the values of an argument structure in field order (0 for NULL): a small call is half over
+    by the time ctypes has filled a structure of 30 fields."""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f"}
+    s = struct.Struct("@" + "".join(code[kind] for _, kind in args._fields_))
+    return struct.Struct(s.format + "x" * (C.sizeof(args) - s.size))
+
+
 def make_options(options):
     """dict of mv_options fields (missing ones keep the library's defaults) -> mv_options, or None for NULL."""
     if not options:
@@ -117,6 +126,28 @@ class mv_profile_row(C.Structure):
     _fields_ = [("name", C.c_char * 192), ("detail", C.c_char * 32), ("launches", C.c_int), ("ms", C.c_double),
                 ("macs_per_frame", C.c_double)]
 
+
+class SequenceOp:
+    """One sequence operator's entry point, taking its argument structure as packed bytes."""
+
+    def __init__(self, name, args, scratch):
+        self.name, self.pack, self.scratch = name, _packer(args).pack, scratch
+        self.fn = self.fn_workspace = None
+
+    def bind(self):
+        vp = C.c_void_p
+        if self.scratch:
+            ws = lib()[self.name + "_workspace"]
+            ws.argtypes, ws.restype = [C.c_char_p], C.c_size_t
+            self.fn_workspace = ws
+        fn = lib()[self.name]  # a function object of its own: the library's attribute takes the structure
+        fn.argtypes = [C.c_char_p, vp, C.c_size_t, vp] if self.scratch else [C.c_char_p, vp]
+        self.fn = fn  # (last: another thread may be looking)
+
+
+GROUP_NORM = SequenceOp("mv_group_norm", mv_group_norm_args, True)
+CAUSAL_CONV = SequenceOp("mv_causal_conv", mv_causal_conv_args, False)
+SELECTIVE_SCAN = SequenceOp("mv_selective_scan", mv_selective_scan_args, True)
 
 _lib = None
 

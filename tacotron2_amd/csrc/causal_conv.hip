@@ -7,33 +7,151 @@
 
 namespace mv {
 
-// One thread per channel of a sequence, walking its frames: the state is read before it is replaced by the same thread.
-template <typename T, int ACT, int K>
-__global__ __launch_bounds__(256) void causal_conv_kernel(Rows<const T> x, Rows<T> y, const void* w, const void* bias,
-                                                          bool w32, const T* state_in, T* state_out,
-                                                          const int32_t* lengths, int B, int Tmax, int C, float slope) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)B * C) return;
-    const int b = (int)(i / C), c = (int)(i % C), len = seq_frames(lengths, b, Tmax);
-    float win[K], wk[K];
-    for (int k = 0; k < K; ++k) {
-        wk[k] = load_weight<T>(w, w32, c * K + k);
-        win[k] = k && state_in ? (float)state_in[((long long)b * (K - 1) + k - 1) * C + c] : 0.f;
+template <typename T>
+struct CausalParams {
+    Rows<const T> x;
+    Rows<T> y;
+    const void *w, *bias;
+    const T* state_in;
+    T* state_out;
+    const int32_t* lengths;
+    int B, Tmax, C, w32;
+    float slope;
+    int vecs, run, runs;  // vectors of a row, frames a thread walks, threads to a sequence's vector
+};
+
+// V channels at p, or the first `n` of them
+template <typename T, int V>
+__device__ __forceinline__ typename Unaligned<T, V>::type load_some(const T* p, int n) {
+    typename Unaligned<T, V>::type v;
+    if (n == V) return *(const typename Unaligned<T, V>::type*)p;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < n ? p[e] : (T)0.f;
+    return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T* p, typename Unaligned<T, V>::type v, int n) {
+    if (n == V) {
+        *(typename Unaligned<T, V>::type*)p = v;
+        return;
     }
-    const float bc = bias ? load_weight<T>(bias, w32, c) : 0.f;
-    for (int t = 0; t < Tmax; ++t) {
-        float v = 0.f;
-        if (t < len) {
-            for (int k = 0; k + 1 < K; ++k) win[k] = win[k + 1];
-            win[K - 1] = (float)x.row(b, t)[c];
-            v = bc;
-            for (int k = 0; k < K; ++k) v += wk[k] * win[k];
-            v = activate<ACT>(v, slope);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < n) p[e] = v[e];
+}
+
+constexpr int kConvStep = 4;  // frames whose loads are in flight together
+
+// A thread walks `run` frames of V adjacent channels with the K - 1 frames before in registers.  The thread of a sequence's
+// first run also moves the state on: it alone reads state_in, before it writes state_out.
+template <typename T, int ACT, int K, int V>
+__global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
+    typedef typename Unaligned<T, V>::type Vec;
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int cv = (int)(id % p.vecs);
+    const long long rest = id / p.vecs;
+    const int r = (int)(rest % p.runs), b = (int)(rest / p.runs);
+    if (b >= p.B) return;
+    const int c = cv * V, n = min(V, p.C - c), len = seq_frames(p.lengths, b, p.Tmax);
+    const int t0 = r * p.run, t1 = min(t0 + p.run, p.Tmax);
+    const T* from = p.x.row(b, 0) + c;
+    T* to = p.y.row(b, 0) + c;
+
+    Vec carry[K];  // (K - 1 of them)
+    if (K > 1 && r == 0) {
+        const long long s = (long long)b * (K - 1) * p.C + c;
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k) {
+            if (p.state_in) {
+                carry[k] = load_some<T, V>(p.state_in + s + (long long)k * p.C, n);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) carry[k][e] = (T)0.f;
+            }
         }
-        y.row(b, t)[c] = (T)v;
+        if (p.state_out) {
+            Vec next[K];
+#pragma unroll
+            for (int k = 0; k + 1 < K; ++k) {
+                const int at = len + k - (K - 1);  // frame that becomes row k, or a row of the state before
+                if (at >= 0) {
+                    next[k] = load_some<T, V>(from + at * p.x.rs, n);
+                } else {
+                    next[k] = carry[k];
+#pragma unroll
+                    for (int q = 1; q + k < K - 1; ++q)
+                        if (len == q) next[k] = carry[k + q];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k + 1 < K; ++k) store_some<T, V>(p.state_out + s + (long long)k * p.C, next[k], n);
+        }
+    } else if (K > 1 && t0 < len) {
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k) {
+            // (a run is no shorter than K - 1 frames unless it is the only one: t0 - (K - 1) >= 0)
+            carry[k] = load_some<T, V>(from + (t0 - (K - 1) + k) * p.x.rs, n);
+        }
     }
-    if (state_out)
-        for (int k = 1; k < K; ++k) state_out[((long long)b * (K - 1) + k - 1) * C + c] = (T)win[k];
+
+    float w[K * V], bias[V];
+    if (t0 < len) {
+        // a vector's taps lie side by side: [channel][K]
+        if (n == V) {
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                if (p.w32) {
+                    const auto t = *(const typename Unaligned<float, V>::type*)((const float*)p.w + c * K + i * V);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[i * V + e] = t[e];
+                } else {
+                    const auto t = *(const Vec*)((const T*)p.w + c * K + i * V);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[i * V + e] = (float)t[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < K * V; ++i) w[i] = i < n * K ? load_weight<T>(p.w, p.w32, c * K + i) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) bias[e] = p.bias && e < n ? load_weight<T>(p.bias, p.w32, c + e) : 0.f;
+    }
+    float x[K - 1 + kConvStep][V];
+#pragma unroll
+    for (int k = 0; k + 1 < K; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[k][e] = (float)carry[k][e];
+    const int live = min(t1, len);
+    int t = t0;
+    for (; t < live; t += kConvStep) {
+        Vec raw[kConvStep];
+#pragma unroll
+        for (int u = 0; u < kConvStep; ++u)
+            if (t + u < live) raw[u] = load_some<T, V>(from + (t + u) * p.x.rs, n);
+#pragma unroll
+        for (int u = 0; u < kConvStep; ++u) {
+            if (t + u >= live) break;
+            Vec y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                x[K - 1 + u][e] = (float)raw[u][e];
+                float v = bias[e];
+#pragma unroll
+                for (int k = 0; k < K; ++k) v += w[e * K + k] * x[u + k][e];
+                y[e] = (T)activate<ACT>(v, p.slope);
+            }
+            store_some<T, V>(to + (t + u) * p.y.rs, y, n);
+        }
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[k][e] = x[k + kConvStep][e];
+    }
+    Vec zero;
+#pragma unroll
+    for (int e = 0; e < V; ++e) zero[e] = (T)0.f;
+    for (t = max(t0, len); t < t1; ++t) store_some<T, V>(to + t * p.y.rs, zero, n);
 }
 
 template <typename F>
@@ -85,14 +203,21 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
     if (int rc = check_output_rows(who, a->y, a->B, a->T, a->C, a->dtype)) return rc;
     return by_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return by_activation(a->activation, [&](auto act) {
+        constexpr int V = 16 / sizeof(T);
+        CausalParams<T> p{rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->state_in, (T*)a->state_out,
+                        a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (a->C + V - 1) / V, 0, 0};
+        // long runs read few frames twice (K - 1 a run), short ones give more threads: as long as 2^17 of them allow
+        for (p.run = 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;) p.run /= 2;
+        p.runs = (a->T + p.run - 1) / p.run;
+        const long long blocks = ((long long)a->B * p.runs * p.vecs + 255) / 256;
+        if (blocks > 0xffffff) {
+            set_error("%s: too many frames for one call", who);
+            return MV_EINVAL;
+        }
+        return by_activation(a->activation, a->slope, &p.slope, [&](auto act) {
             return by_taps(a->K, [&](auto taps) {
-                const long long n = (long long)a->B * a->C;
-                hipLaunchKernelGGL((causal_conv_kernel<T, decltype(act)::value, decltype(taps)::value>),
-                                   dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                                   rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias,
-                                   a->weight_dtype == MV_DTYPE_F32, (const T*)a->state_in, (T*)a->state_out, a->lengths,
-                                   a->B, a->T, a->C, a->slope);
+                hipLaunchKernelGGL((causal_conv_kernel<T, decltype(act)::value, decltype(taps)::value, V>),
+                                   dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
                 MV_HIP(hipGetLastError());
                 return MV_OK;
             });

@@ -2,7 +2,17 @@
 //
 //   y = act((x - m) / sqrt(v + eps) * w_c + b_c),  m and v over (t < len, c in group), or over a frame's group alone
 //
-// HBM-bound: x once in, y once out.
+// HBM-bound: x once in, y once out.  The variance is a sum of squared distances from a mean that is already known (sums of
+// squares lose it where the mean is far from zero), so what is normalised has to be looked at twice: it stays in registers
+// between the two looks wherever it fits.
+//
+//   frame_norm_kernel     per frame, groups of up to 64 * 8 vectors: L lanes hold a group
+//   group_norm_kernel     a sequence's group(s) in one block's registers: one read, one write, one launch
+//   group_stats_kernel +  a sequence in pieces: count, mean and squared distances of each piece that a block's registers
+//   group_apply_kernel    hold; then the pieces are put together and x is read a second time
+//   wide_norm_kernel      what none of them holds: groups of more channels than a block holds at once
+//
+// A vector is the largest power of two of channels, 16 bytes at most, that divides a group: it never holds two groups.
 #include "sequence.h"
 
 namespace mv {
@@ -20,8 +30,8 @@ int check_sequence(const char* who, int B, int T, int C, int dtype) {
 }
 
 int check_rows(const char* who, const char* what, const mv_rows& r, int dtype) {
-    if (!r.ptr || ((uintptr_t)r.ptr % dtype_size(dtype)) != 0 || r.batch_stride < 0 || r.row_stride < 0) {
-        set_error("%s: %s needs an aligned pointer and strides >= 0", who, what);
+    if (!r.ptr || ((uintptr_t)r.ptr % dtype_size(dtype)) != 0 || r.batch_stride < 0 || r.row_stride < 0 || r.row_stride > 1 << 25) {
+        set_error("%s: %s needs an aligned pointer, strides >= 0 and a row stride of at most 2^25", who, what);
         return MV_EINVAL;
     }
     return MV_OK;
@@ -47,25 +57,338 @@ int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, in
     return MV_OK;
 }
 
-// One block per group of a sequence (or of a frame): mean, then the squared distances from it, then the result.
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void group_norm_kernel(Rows<const T> x, Rows<T> y, const void* w, const void* bias,
-                                                         bool w32, const int32_t* lengths, int Tmax, int C, int G,
-                                                         int per_frame, float slope, float eps) {
-    __shared__ float red[256];
-    const int Cg = C / G;
-    long long item = blockIdx.x;
-    const int g = item % G;
-    item /= G;
-    int t0 = 0, t1 = Tmax;
-    if (per_frame) {
-        t0 = item % Tmax;
-        t1 = t0 + 1;
-        item /= Tmax;
+template <typename T>
+struct NormParams {
+    Rows<const T> x;
+    Rows<T> y;
+    const void *w, *b;
+    const int32_t* lengths;
+    float *n, *mean, *m2;  // pieces' statistics [B][G][pieces]
+    int B, Tmax, C, G, w32;
+    float slope, eps;
+    int tile, tiles;     // vectors of a row to a block, blocks to a row
+    int piece, pieces;   // frames to a block, blocks to a sequence
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_weights(const void* w, bool w32, int c, float none, float (&v)[V]) {
+    if (!w) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = none;
+    } else if (w32) {
+        const auto t = *(const typename Unaligned<float, V>::type*)((const float*)w + c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = t[e];
+    } else {
+        const auto t = *(const typename Unaligned<T, V>::type*)((const T*)w + c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (float)t[e];
     }
-    const int b = (int)item, len = seq_frames(lengths, b, Tmax);
-    const int c0 = g * Cg, end = min(t1, len);
-    const long long n = (long long)max(0, end - t0) * Cg, all = (long long)(t1 - t0) * Cg;
+}
+
+// (x - mean) * rstd * w + b of one vector
+template <typename T, int V, int ACT>
+__device__ __forceinline__ typename Unaligned<T, V>::type normalise(typename Unaligned<T, V>::type x, float mean, float rstd,
+                                                                    const float (&w)[V], const float (&b)[V], float slope) {
+    typename Unaligned<T, V>::type y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = (T)activate<ACT>(((float)x[e] - mean) * rstd * w[e] + b[e], slope);
+    return y;
+}
+
+// A vector as it was loaded, for the compiler a new value: what is computed from it is computed again rather than kept, and
+// the registers that hold a tile hold its 16-bit elements, not their float32 conversions.
+template <typename Vec>
+__device__ __forceinline__ Vec forget(Vec v) {
+    struct Words {
+        unsigned w[(sizeof(Vec) + 3) / 4];
+    } u{};
+    __builtin_memcpy(&u, &v, sizeof(Vec));
+#pragma unroll
+    for (unsigned& w : u.w) asm volatile("" : "+v"(w));
+    __builtin_memcpy(&v, &u, sizeof(Vec));
+    return v;
+}
+
+// The sum of `v` over the threads of each group of the block.  Threads stand row-major over [rows][tile] vectors, a group is
+// `gv` adjacent vectors of every row; a wave adds up a group's values, `red` holds one float a thread and one a group.
+// Every thread of the block calls it; the order of additions depends on the layout alone.
+__device__ __forceinline__ float group_total(float v, float* red, int rows, int tile, int gv, int mine) {
+    const int groups = tile / gv, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+    float* res = red + blockDim.x;
+    red[threadIdx.x] = v;
+    __syncthreads();
+    for (int g = threadIdx.x >> 6; g < groups; g += waves) {
+        float s = 0.f;
+        for (int i = lane; i < rows * gv; i += 64) s += red[i / gv * tile + g * gv + i % gv];
+#pragma unroll
+        for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m);
+        if (lane == 0) res[g] = s;
+    }
+    __syncthreads();
+    const float r = res[mine];
+    __syncthreads();
+    return r;
+}
+
+// A block's thread on a tile of vectors of a row: which vector, which rows (row, row + rows, ...), which group of the tile.
+// Addresses are a base that the block shares plus a 32-bit offset of the thread (the plan sees to it that it fits).
+template <typename T, int V>
+struct Place {
+    int row, rows, c, mine, gv;
+    bool in;  // false: a thread without a row, or past the last vector of a row; it loads what its neighbour does
+
+    __device__ __forceinline__ Place(const NormParams<T>& p) {
+        const int tile0 = blockIdx.x * p.tile, v = threadIdx.x % p.tile;
+        gv = p.C / p.G / V;
+        rows = blockDim.x / p.tile;
+        row = min((int)threadIdx.x / p.tile, rows - 1);
+        in = threadIdx.x < rows * p.tile && tile0 + v < p.C / V;
+        c = min(tile0 + v, p.C / V - 1) * V;
+        mine = v / gv;
+    }
+    // frame t0 + row + i * rows; frames from `end` on: frame end - 1
+    template <typename P>
+    __device__ __forceinline__ P* at(P* frame0, long long rs, int t0, int i, int end) const {
+        const unsigned first = (unsigned)(row * (int)rs + c) * (unsigned)sizeof(T);
+        if (t0 + (i + 1) * rows <= end) return (P*)((char*)(frame0 + (t0 + (long long)i * rows) * rs) + first);
+        const int r = min(row + i * rows, end - 1 - t0);
+        return (P*)((char*)(frame0 + t0 * rs) + (unsigned)(r * (int)rs + c) * (unsigned)sizeof(T));
+    }
+};
+
+// Frames [t0, t1) of a tile in the block's registers, NI vectors to a thread, and the statistics of the thread's group.
+template <typename T, int V, int NI>
+struct Held {
+    typedef typename Unaligned<T, V>::type Vec;
+    Vec x[NI];
+    float mean, m2;
+
+    // count: frames * channels of the group
+    __device__ __forceinline__ void take(const NormParams<T>& p, const Place<T, V>& at, int b, int t0, int t1, float count,
+                                         float* red) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[i] = *(const Vec*)at.at(p.x.row(b, 0), p.x.rs, t0, i, t1);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (at.in && t0 + at.row + i * at.rows < t1)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += (float)x[i][e];
+        mean = group_total(s, red, at.rows, p.tile, at.gv, at.mine) / count;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[i] = forget(x[i]);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (at.in && t0 + at.row + i * at.rows < t1)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = (float)x[i][e] - mean;
+                    s += d * d;
+                }
+        m2 = group_total(s, red, at.rows, p.tile, at.gv, at.mine);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[i] = forget(x[i]);
+    }
+};
+
+constexpr int kNormThreads = 1024;
+
+// Grid (tiles, sequences): whole groups of a whole sequence.
+template <typename T, int V, int NI, int ACT>
+__global__ __launch_bounds__(kNormThreads) void group_norm_kernel(NormParams<T> p) {
+    __shared__ float red[2 * kNormThreads];
+    typedef typename Unaligned<T, V>::type Vec;
+    const Place<T, V> at(p);
+    Held<T, V, NI> h;
+    for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+        const int len = seq_frames(p.lengths, b, p.Tmax);
+        const float count = (float)len * (float)(p.C / p.G);
+        if (len) h.take(p, at, b, 0, len, count, red);
+        const float rstd = 1.f / sqrtf(h.m2 / count + p.eps);
+        float w[V], bias[V];
+        load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
+        load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int t = at.row + i * at.rows;
+            Vec y;
+            if (t < len) {
+                y = normalise<T, V, ACT>(h.x[i], h.mean, rstd, w, bias, p.slope);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = (T)0.f;
+            }
+            if (at.in && t < p.Tmax) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, 0, i, p.Tmax) = y;
+            __builtin_amdgcn_sched_barrier(0);  // one vector after the other: the registers hold the tile, not 16 results
+        }
+    }
+}
+
+// Grid (tiles, pieces, sequences): statistics of a piece of a sequence.
+template <typename T, int V, int NI>
+__global__ __launch_bounds__(kNormThreads) void group_stats_kernel(NormParams<T> p) {
+    __shared__ float red[2 * kNormThreads];
+    const Place<T, V> at(p);
+    Held<T, V, NI> h;
+    for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
+        const int len = seq_frames(p.lengths, b, p.Tmax);
+        const int t0 = blockIdx.y * p.piece, t1 = min(t0 + p.piece, len);
+        const int Cg = p.C / p.G;
+        const float count = t1 > t0 ? (float)(t1 - t0) * (float)Cg : 0.f;
+        h.mean = h.m2 = 0.f;
+        if (t1 > t0) h.take(p, at, b, t0, t1, count, red);
+        if (at.in && at.row == 0 && at.c % Cg == 0) {
+            const long long i = ((long long)b * p.G + at.c / Cg) * p.pieces + blockIdx.y;
+            p.n[i] = count;
+            p.mean[i] = h.mean;
+            p.m2[i] = h.m2;
+        }
+    }
+}
+
+// Mean and 1 / sqrt(variance + eps) of a group from its pieces, by one wave: sum n_i m_i / n, then the pieces' own squared
+// distances and those of their means.
+__device__ __forceinline__ void join_pieces(const float* n, const float* mean, const float* m2, int pieces, float eps,
+                                            float* out_mean, float* out_rstd) {
+    const int lane = threadIdx.x & 63;
+    float N = 0.f, s = 0.f;
+    for (int i = lane; i < pieces; i += 64) N += n[i], s += n[i] * mean[i];
+#pragma unroll
+    for (int m = 32; m; m >>= 1) N += __shfl_xor(N, m), s += __shfl_xor(s, m);
+    const float mu = s / N;
+    float q = 0.f;
+    for (int i = lane; i < pieces; i += 64) {
+        const float d = mean[i] - mu;
+        q += m2[i] + (n[i] > 0.f ? n[i] * d * d : 0.f);
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) q += __shfl_xor(q, m);
+    if (lane == 0) *out_mean = mu, *out_rstd = 1.f / sqrtf(q / N + eps);
+}
+
+// Grid (tiles, pieces, sequences), the last ones first: what the statistics read last is still in the caches.  `piece` is
+// this launch's own, a multiple of 4 * rows frames.
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T> p) {
+    __shared__ float stat[2 * kNormThreads];
+    typedef typename Unaligned<T, V>::type Vec;
+    const Place<T, V> at(p);
+    float w[V], bias[V];
+    load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
+    load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
+    const int Cg = p.C / p.G, g0 = blockIdx.x * p.tile * V / Cg, groups = p.tile * V / Cg;
+    const int piece = gridDim.y - 1 - blockIdx.y;
+    for (int bb = blockIdx.z; bb < p.B; bb += gridDim.z) {
+        const int b = p.B - 1 - bb, len = seq_frames(p.lengths, b, p.Tmax);
+        const int t0 = piece * p.piece, te = min(t0 + p.piece, p.Tmax), live = min(te, len);
+        __syncthreads();
+        if (t0 < live)
+            for (int g = threadIdx.x >> 6; g < groups; g += blockDim.x >> 6)
+                if (g0 + g < p.G) {
+                    const long long i = ((long long)b * p.G + g0 + g) * p.pieces;
+                    join_pieces(p.n + i, p.mean + i, p.m2 + i, p.pieces, p.eps, &stat[g], &stat[kNormThreads + g]);
+                }
+        __syncthreads();
+        const float mean = stat[at.mine], rstd = stat[kNormThreads + at.mine];
+        for (int t = t0; t < te; t += 4 * at.rows) {
+            Vec x[4];
+            if (t < live) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = *(const Vec*)at.at(p.x.row(b, 0), p.x.rs, t, i, live);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int f = t + at.row + i * at.rows;
+                Vec y;
+                if (f < live) {
+                    y = normalise<T, V, ACT>(x[i], mean, rstd, w, bias, p.slope);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[e] = (T)0.f;
+                }
+                if (at.in && f < te) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, t, i, te) = y;
+            }
+        }
+    }
+}
+
+// Each frame's groups by themselves: L lanes to a group, NI vectors to a lane.  A slot of L lanes keeps its group (and its
+// weights) and walks the frames.
+template <typename T, int V, int NI, int ACT>
+__global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L, long long slots) {
+    typedef typename Unaligned<T, V>::type Vec;
+    const long long slot = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    if (slot >= slots) return;  // (whole slots leave: L divides 64)
+    const int l = threadIdx.x & (L - 1), Cg = p.C / p.G, nv = Cg / V, g = (int)(slot % p.G);
+    float w[NI][V], bias[NI][V];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int c = g * Cg + min(l + i * L, nv - 1) * V;
+        load_weights<T, V>(p.w, p.w32, c, 1.f, w[i]);
+        load_weights<T, V>(p.b, p.w32, c, 0.f, bias[i]);
+    }
+    const long long frames = (long long)p.B * p.Tmax;
+    for (long long f = slot / p.G; f < frames; f += slots / p.G) {
+        const int b = (int)(f / p.Tmax), t = (int)(f - (long long)b * p.Tmax);
+        T* to = p.y.row(b, t) + g * Cg;
+        if (t >= seq_frames(p.lengths, b, p.Tmax)) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                Vec y;
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = (T)0.f;
+                if (l + i * L < nv) *(Vec*)(to + (l + i * L) * V) = y;
+            }
+            continue;
+        }
+        const T* from = p.x.row(b, t) + g * Cg;
+        Vec x[NI];
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (l + i * L < nv) x[i] = *(const Vec*)(from + (l + i * L) * V);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (l + i * L < nv)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += (float)x[i][e];
+        for (int m = L >> 1; m; m >>= 1) s += __shfl_xor(s, m);
+        const float mean = s / (float)Cg;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (l + i * L < nv)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = (float)x[i][e] - mean;
+                    s += d * d;
+                }
+        for (int m = L >> 1; m; m >>= 1) s += __shfl_xor(s, m);
+        const float rstd = 1.f / sqrtf(s / (float)Cg + p.eps);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (l + i * L < nv) *(Vec*)(to + (l + i * L) * V) = normalise<T, V, ACT>(x[i], mean, rstd, w[i], bias[i], p.slope);
+    }
+}
+
+// One block per group of a sequence (or of a frame), element by element: groups that no block's registers hold.
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void wide_norm_kernel(NormParams<T> p, int per_frame) {
+    __shared__ float red[256];
+    const int Cg = p.C / p.G;
+    long long item = blockIdx.x;
+    const int g = item % p.G;
+    item /= p.G;
+    int t0 = 0, t1 = p.Tmax;
+    if (per_frame) {
+        t0 = item % p.Tmax;
+        t1 = t0 + 1;
+        item /= p.Tmax;
+    }
+    const int b = (int)item, len = seq_frames(p.lengths, b, p.Tmax), c0 = g * Cg, end = min(t1, len);
+    const float count = (float)max(0, end - t0) * (float)Cg;
     auto total = [&](float v) {
         red[threadIdx.x] = v;
         __syncthreads();
@@ -78,24 +401,157 @@ __global__ __launch_bounds__(256) void group_norm_kernel(Rows<const T> x, Rows<T
         return r;
     };
     float s = 0.f;
-    for (long long i = threadIdx.x; i < n; i += 256) s += (float)x.row(b, t0 + (int)(i / Cg))[c0 + i % Cg];
-    const float mean = total(s) / (float)n;
+    for (int t = t0; t < end; ++t) {
+        float row = 0.f;  // (a row's sum by itself: a thread adds up at most its channels plus its rows in one chain)
+        for (int c = threadIdx.x; c < Cg; c += 256) row += (float)p.x.row(b, t)[c0 + c];
+        s += row;
+    }
+    const float mean = total(s) / count;
     s = 0.f;
-    for (long long i = threadIdx.x; i < n; i += 256) {
-        const float d = (float)x.row(b, t0 + (int)(i / Cg))[c0 + i % Cg] - mean;
-        s += d * d;
-    }
-    const float r = 1.f / sqrtf(total(s) / (float)n + eps);
-    for (long long i = threadIdx.x; i < all; i += 256) {
-        const int c = c0 + (int)(i % Cg), t = t0 + (int)(i / Cg);
-        float v = 0.f;
-        if (i < n) {
-            v = ((float)x.row(b, t)[c] - mean) * r;
-            v = v * (w ? load_weight<T>(w, w32, c) : 1.f) + (bias ? load_weight<T>(bias, w32, c) : 0.f);
-            v = activate<ACT>(v, slope);
+    for (int t = t0; t < end; ++t) {
+        float row = 0.f;
+        for (int c = threadIdx.x; c < Cg; c += 256) {
+            const float d = (float)p.x.row(b, t)[c0 + c] - mean;
+            row += d * d;
         }
-        y.row(b, t)[c] = (T)v;
+        s += row;
     }
+    const float rstd = 1.f / sqrtf(total(s) / count + p.eps);
+    for (int t = t0; t < t1; ++t)
+        for (int c = c0 + threadIdx.x; c < c0 + Cg; c += 256) {
+            float v = 0.f;
+            if (t < end) {
+                v = ((float)p.x.row(b, t)[c] - mean) * rstd;
+                v = v * (p.w ? load_weight<T>(p.w, p.w32, c) : 1.f) + (p.b ? load_weight<T>(p.b, p.w32, c) : 0.f);
+                v = activate<ACT>(v, p.slope);
+            }
+            p.y.row(b, t)[c] = (T)v;
+        }
+}
+
+// --- host side -----------------------------------------------------------------------------------------------------
+enum { NORM_FRAME, NORM_HELD, NORM_PIECES, NORM_WIDE };
+struct NormPlan {
+    int kind, V, NI, threads, tile, tiles, piece, pieces, apply_piece, L;
+    size_t bytes;
+};
+
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+static int pow2_at_least(int v, int most) {
+    int p = 1;
+    while (p < v && p < most) p *= 2;
+    return p;
+}
+
+static NormPlan norm_plan(const mv_group_norm_args* a) {
+    NormPlan s{};
+    const int Cg = a->C / a->groups, size = (int)dtype_size(a->dtype);
+    s.V = 16 / size;
+    while (Cg % s.V) s.V /= 2;
+    const int gv = Cg / s.V, row = a->C / s.V;
+    s.kind = NORM_WIDE;
+    if (a->per_frame) {
+        if (gv > 64 * 8) return s;
+        s.kind = NORM_FRAME;
+        s.L = pow2_at_least(gv, 64);
+        s.NI = pow2_at_least(ceil_div(gv, s.L), 8);
+        return s;
+    }
+    if (gv > kNormThreads) return s;
+    const long long far = std::max(a->x.row_stride, a->y.row_stride);
+    auto fits = [&](long long frames) { return (frames * far + a->C) * size < 1ll << 31; };  // Place's offsets
+    // whole groups side by side until a row of the tile is a 128-byte line
+    s.tile = gv;
+    while (s.tile * s.V * size < 128 && s.tile + gv <= std::min(row, kNormThreads)) s.tile += gv;
+    for (int threads = 256; threads <= kNormThreads; threads *= 2) {
+        if (threads < s.tile) continue;
+        const int n = ceil_div(a->T, threads / s.tile);
+        if (n <= (threads < kNormThreads ? 4 : 16) && fits(threads / s.tile * 16)) {
+            s.kind = NORM_HELD;
+            s.threads = threads;
+            s.NI = n <= 1 ? 1 : n <= 4 ? 4 : 16;
+            s.tiles = ceil_div(row, s.tile);
+            return s;
+        }
+    }
+    // pieces: blocks of 1024 threads, as large as leaves two for each CU
+    s.threads = kNormThreads;
+    s.tiles = ceil_div(row, s.tile);
+    const int rows = s.threads / s.tile;
+    for (s.NI = 16;; s.NI = 4) {
+        s.piece = rows * s.NI;
+        s.pieces = ceil_div(a->T, s.piece);
+        if (s.NI == 4 || (long long)s.tiles * s.pieces * a->B >= 512) break;
+    }
+    s.apply_piece = rows * 8;
+    if (ceil_div(a->T, s.apply_piece) > 65535 || !fits(rows * s.NI)) return s;
+    s.kind = NORM_PIECES;
+    s.bytes = ((size_t)a->B * a->groups * s.pieces * 3 * 4 + 255) / 256 * 256;
+    return s;
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// calls f(V, NI) with the plan's vector and count as constants
+template <typename T, typename F>
+static int by_plan(const NormPlan& s, F&& f) {
+    auto by_count = [&](auto v) {
+        switch (s.NI) {
+            case 1: return f(v, Int<1>());
+            case 2: return f(v, Int<2>());
+            case 4: return f(v, Int<4>());
+            case 8: return f(v, Int<8>());
+            default: return f(v, Int<16>());
+        }
+    };
+    switch (s.V) {
+        case 1: return by_count(Int<1>());
+        case 2: return by_count(Int<2>());
+        case 4: return by_count(Int<4>());
+        default: return by_count(Int<(sizeof(T) == 2 ? 8 : 4)>());
+    }
+}
+
+template <typename T, int ACT>
+static int launch_norm(const mv_group_norm_args* a, const NormPlan& s, NormParams<T> p, hipStream_t stream) {
+    const unsigned B16 = (unsigned)std::min(a->B, 65535);
+    if (s.kind == NORM_WIDE) {
+        const long long items = (long long)a->B * a->groups * (a->per_frame ? a->T : 1);
+        if (items > 0xffffff) {
+            set_error("mv_group_norm: more than 2^24 groups of over %d channels", a->per_frame ? 512 * s.V : kNormThreads * s.V);
+            return MV_EINVAL;
+        }
+        hipLaunchKernelGGL((wide_norm_kernel<T, ACT>), dim3((unsigned)items), dim3(256), 0, stream, p, a->per_frame);
+        MV_HIP(hipGetLastError());
+        return MV_OK;
+    }
+    return by_plan<T>(s, [&](auto v, auto n) {
+        constexpr int V = decltype(v)::value, NI = decltype(n)::value;
+        if (s.kind == NORM_FRAME) {
+            if constexpr (NI <= 8) {
+                const long long frames = (long long)a->B * a->T, most = 2048ll * 256 / s.L / a->groups;
+                const long long slots = std::min(frames, std::max(1ll, most)) * a->groups;
+                hipLaunchKernelGGL((frame_norm_kernel<T, V, NI, ACT>), dim3((unsigned)((slots * s.L + 255) / 256)), dim3(256), 0,
+                                   stream, p, s.L, slots);
+            }
+        } else if constexpr (NI == 1 || NI == 4 || NI == 16) {
+            p.tile = s.tile;
+            if (s.kind == NORM_HELD) {
+                hipLaunchKernelGGL((group_norm_kernel<T, V, NI, ACT>), dim3(s.tiles, B16), dim3(s.threads), 0, stream, p);
+            } else if constexpr (NI > 1) {
+                p.piece = s.piece;
+                p.pieces = s.pieces;
+                hipLaunchKernelGGL((group_stats_kernel<T, V, NI>), dim3(s.tiles, s.pieces, B16), dim3(s.threads), 0, stream, p);
+                MV_HIP(hipGetLastError());
+                p.piece = s.apply_piece;
+                hipLaunchKernelGGL((group_apply_kernel<T, V, ACT>), dim3(s.tiles, ceil_div(a->T, s.apply_piece), B16),
+                                   dim3(s.threads), 0, stream, p);
+            }
+        }
+        MV_HIP(hipGetLastError());
+        return MV_OK;
+    });
 }
 
 }  // namespace mv
@@ -127,8 +583,8 @@ static int check_group_norm(const mv_group_norm_args* a) {
 extern "C" {
 
 size_t mv_group_norm_workspace(const mv_group_norm_args* a) {
-    if (check_group_norm(a)) return 0;
-    return 0;
+    if (check_group_norm(a) || a->B == 0 || a->T == 0) return 0;
+    return norm_plan(a).bytes;
 }
 
 int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -136,20 +592,31 @@ int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace
     if (a->B == 0 || a->T == 0) return MV_OK;
     if (int rc = check_rows("mv_group_norm", "x", a->x, a->dtype)) return rc;
     if (int rc = check_output_rows("mv_group_norm", a->y, a->B, a->T, a->C, a->dtype)) return rc;
-    const long long items = (long long)a->B * a->groups * (a->per_frame ? a->T : 1);
-    if (items > 0xffffff) {
-        set_error("mv_group_norm: too many groups");
-        return MV_EINVAL;
+    const NormPlan plan = norm_plan(a);
+    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 255) != 0)) {
+        set_error("mv_group_norm: workspace: need %zu bytes, 256-byte aligned (got %zu)", plan.bytes, workspace_bytes);
+        return MV_ENOMEM;
     }
     return by_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return by_activation(a->activation, [&](auto act) {
-            hipLaunchKernelGGL((group_norm_kernel<T, decltype(act)::value>), dim3((unsigned)items), dim3(256), 0,
-                               (hipStream_t)stream, rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias,
-                               a->weight_dtype == MV_DTYPE_F32, a->lengths, a->T, a->C, a->groups, a->per_frame, a->slope,
-                               a->eps);
-            MV_HIP(hipGetLastError());
-            return MV_OK;
+        NormParams<T> p{};
+        p.x = rows_of<const T>(a->x);
+        p.y = rows_of<T>(a->y);
+        p.w = a->weight;
+        p.b = a->bias;
+        p.lengths = a->lengths;
+        const size_t n = (size_t)a->B * a->groups * plan.pieces;
+        p.n = (float*)workspace;
+        p.mean = p.n + n;
+        p.m2 = p.mean + n;
+        p.B = a->B;
+        p.Tmax = a->T;
+        p.C = a->C;
+        p.G = a->groups;
+        p.w32 = a->weight_dtype == MV_DTYPE_F32;
+        p.eps = a->eps;
+        return by_activation(a->activation, a->slope, &p.slope, [&](auto act) {
+            return launch_norm<T, decltype(act)::value>(a, plan, p, (hipStream_t)stream);
         });
     });
 }

@@ -18,6 +18,12 @@ inline Rows<T> rows_of(const mv_rows& r) {
     return Rows<T>{(T*)r.ptr, (long long)r.batch_stride, (long long)r.row_stride};
 }
 
+// a vector of N elements at any address an element may have (the hardware's vector loads and stores need no more)
+template <typename T, int N>
+struct Unaligned {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
 constexpr float kLog2e = 1.44269504088896341f;
 
 // sigmoid and its relatives on the hardware exp2 and reciprocal (1 ulp each): exp2 overflowing to inf gives the right 0
@@ -41,8 +47,7 @@ template <int ACT>
 __device__ __forceinline__ float activate(float v, float slope) {
     if (ACT == MV_ACT_SILU) return v * sigmoidf(v);
     if (ACT == MV_ACT_LRELU) return v < 0.f ? (slope == 0.f ? 0.f : slope * v) : v;
-    if (ACT == MV_ACT_TANH) return tanh_accurate(v);
-    return v;
+    return tanh_accurate(v);
 }
 
 // weights are float32 or of the data's type
@@ -62,12 +67,14 @@ inline int by_dtype(int dtype, F&& f) {
     set_error("unknown dtype %d", dtype);
     return MV_EINVAL;
 }
+// no activation is a leaky_relu of slope 1
 template <typename F>
-inline int by_activation(int act, F&& f) {
+inline int by_activation(int act, float slope, float* use_slope, F&& f) {
+    *use_slope = act == MV_ACT_NONE ? 1.f : slope;
     switch (act) {
-        case MV_ACT_NONE: return f(std::integral_constant<int, MV_ACT_NONE>());
-        case MV_ACT_SILU: return f(std::integral_constant<int, MV_ACT_SILU>());
+        case MV_ACT_NONE:
         case MV_ACT_LRELU: return f(std::integral_constant<int, MV_ACT_LRELU>());
+        case MV_ACT_SILU: return f(std::integral_constant<int, MV_ACT_SILU>());
         case MV_ACT_TANH: return f(std::integral_constant<int, MV_ACT_TANH>());
     }
     set_error("unknown activation %d", act);

@@ -21,8 +21,6 @@ into a HIP graph.  These are synthesis-time layers: inputs that require a gradie
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _native
@@ -42,29 +40,22 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, slo
                   ahead and is the same in a whole call as frame by frame
     activation    None, "silu", "relu", "leaky_relu" (with `slope`) or "tanh"
     """
-    x, B, T, ch, squeeze = _data("group_norm", "x", x)
+    x, shape, B, T, ch, sb, st = _data("group_norm", "x", x)
     if groups < 1 or ch % groups:
         raise RuntimeError(f"group_norm: {ch} channels do not split into {groups} groups")
     if not 0.0 <= eps < float("inf"):
         raise RuntimeError("group_norm: eps must be finite and not negative")
     act, slope = _activation("group_norm", activation, slope)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        weight, bias = weight.float(), bias.float()
-    weight, bias = _weights("group_norm", x, (("weight", weight, (ch,)), ("bias", bias, (ch,))))
-    _no_grad("group_norm", x, weight, bias)
-    y = x.new_empty((B, T, ch))
-    if y.numel() == 0:
-        return y
-    lengths = _lengths(lengths, B, T, x)
-    sx = x.stride()
-    w = weight if weight is not None else bias
-    a = _native.mv_group_norm_args(
-        x.data_ptr(), sx[0], sx[-2] if not squeeze else 0, y.data_ptr(), T * ch, ch,
-        weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
-        lengths.data_ptr() if lengths is not None else None, B, T, ch, groups, _DTYPES[x.dtype],
-        _DTYPES[w.dtype] if w is not None else 0, 1 if per_frame else 0, act, slope, eps)
-    _call("mv_group_norm", a, x, True)
-    return y[:, 0] if squeeze else y
+    weight, bias, wtype = _weights("group_norm", x, weight, (ch,), bias, ch)
+    if torch.is_grad_enabled():
+        _no_grad("group_norm", x, weight, bias)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if B and T:
+        lengths = _lengths(lengths, B, T, x)
+        _call(_native.GROUP_NORM, x, T > 1, _native.GROUP_NORM.pack(
+            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, _ptr(weight), _ptr(bias), _ptr(lengths), B, T, ch, groups,
+            _DTYPES[x.dtype], wtype, 1 if per_frame else 0, act, slope, eps))
+    return y
 
 
 def causal_conv(x, weight, bias=None, activation=None, slope=0.1, state=None, state_out=None, lengths=None):
@@ -75,29 +66,23 @@ def causal_conv(x, weight, bias=None, activation=None, slope=0.1, state=None, st
     weight     [C, K] or [C, 1, K] (a depthwise `torch.nn.Conv1d`'s), 1 <= K <= 8, float32 or x's type; bias [C] or None
     state      [B, K - 1, C] of x's type, the frames before the first, oldest first (None: zeros); state_out likewise
     """
-    x, B, T, ch, squeeze = _data("causal_conv", "x", x)
-    if weight.dim() == 3 and weight.size(1) == 1:
-        weight = weight[:, 0]
-    if weight.dim() != 2 or weight.size(0) != ch or not 1 <= weight.size(1) <= MAX_TAPS:
-        raise RuntimeError(f"causal_conv: expected a weight [{ch}, K] with 1 <= K <= {MAX_TAPS}, got {tuple(weight.shape)}")
-    K = weight.size(1)
+    x, shape, B, T, ch, sb, st = _data("causal_conv", "x", x)
+    w = weight.shape
+    K = w[-1] if len(w) > 1 else 0
+    if not (w == (ch, K) or w == (ch, 1, K)) or not 1 <= K <= MAX_TAPS:
+        raise RuntimeError(f"causal_conv: expected a weight [{ch}, K] with 1 <= K <= {MAX_TAPS}, got {tuple(w)}")
     act, slope = _activation("causal_conv", activation, slope)
-    if bias is not None and weight.dtype != bias.dtype:
-        weight, bias = weight.float(), bias.float()
-    weight, bias = _weights("causal_conv", x, (("weight", weight, (ch, K)), ("bias", bias, (ch,))))
-    state, state_out = _states("causal_conv", x, state, state_out, (B, K - 1, ch), x.dtype)
-    _no_grad("causal_conv", x, weight, bias, state, state_out)
-    y = x.new_empty((B, T, ch))
+    weight, bias, wtype = _weights("causal_conv", x, weight, w, bias, ch)
+    _states("causal_conv", x, state, state_out, (B, K - 1, ch), x.dtype)
+    if torch.is_grad_enabled():
+        _no_grad("causal_conv", x, weight, bias, state, state_out)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
     if B and (T or state_out is not None):
         lengths = _lengths(lengths, B, T, x)
-        sx = x.stride()
-        a = _native.mv_causal_conv_args(
-            x.data_ptr(), sx[0], sx[-2] if not squeeze else 0, y.data_ptr(), T * ch, ch, weight.data_ptr(),
-            bias.data_ptr() if bias is not None else None, state.data_ptr() if state is not None else None,
-            state_out.data_ptr() if state_out is not None else None, lengths.data_ptr() if lengths is not None else None,
-            B, T, ch, K, _DTYPES[x.dtype], _DTYPES[weight.dtype], act, slope)
-        _call("mv_causal_conv", a, x, False)
-    return y[:, 0] if squeeze else y
+        _call(_native.CAUSAL_CONV, x, False, _native.CAUSAL_CONV.pack(
+            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(state_out),
+            _ptr(lengths), B, T, ch, K, _DTYPES[x.dtype], wtype, act, slope))
+    return y
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False, state=None, state_out=None,
@@ -114,64 +99,74 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     state         [B, D, N] float32 (None: zeros); state_out likewise
     u, delta, z, B, C share one type.
     """
-    u, nb, T, ch, squeeze = _data("selective_scan", "u", u)
+    u, shape, nb, T, ch, sb, st = _data("selective_scan", "u", u)
     for name, t in (("delta", delta), ("z", z)):
-        if t is not None and t.shape != u.shape:
-            raise RuntimeError(f"selective_scan: {name} has shape {tuple(t.shape)}, u {tuple(u.shape)}")
-    if A.dim() != 2 or A.size(0) != ch or not 1 <= A.size(1) <= MAX_STATES:
-        raise RuntimeError(f"selective_scan: expected A [{ch}, N] with 1 <= N <= {MAX_STATES}, got {tuple(A.shape)}")
-    N = A.size(1)
-    lead = u.dim() - 1
-    G = B.size(-2) if B.dim() == lead + 2 else 1
-    for name, t in (("B", B), ("C", C)):
-        if (t.shape[:lead] != u.shape[:lead] or t.size(-1) != N or t.dim() not in (lead + 1, lead + 2)
-                or (t.size(-2) if t.dim() == lead + 2 else 1) != G):
-            raise RuntimeError(f"selective_scan: {name} must be {list(u.shape[:lead])} + [{N}] or [G, {N}], B and C alike, got "
-                               f"{tuple(t.shape)}")
+        if t is not None and t.shape != shape:
+            raise RuntimeError(f"selective_scan: {name} has shape {tuple(t.shape)}, u {tuple(shape)}")
+    a = A.shape
+    if len(a) != 2 or a[0] != ch or not 1 <= a[1] <= MAX_STATES:
+        raise RuntimeError(f"selective_scan: expected A [{ch}, N] with 1 <= N <= {MAX_STATES}, got {tuple(a)}")
+    N = a[1]
+    lead, m = shape[:-1], B.shape
+    G = m[-2] if len(m) == len(shape) + 1 else 1
+    if C.shape != m or not (m == (*lead, N) or m == (*lead, G, N)):
+        raise RuntimeError(f"selective_scan: B and C must be {list(lead)} + [{N}] or [G, {N}], got {tuple(m)} and "
+                           f"{tuple(C.shape)}")
     if G < 1 or ch % G:
         raise RuntimeError(f"selective_scan: {ch} channels do not split into {G} groups")
+    dev = u.get_device()
     for name, t in (("delta", delta), ("z", z), ("B", B), ("C", C)):
-        if t is not None and (t.dtype != u.dtype or t.get_device() != u.get_device()):
+        if t is not None and (t.dtype != u.dtype or t.get_device() != dev):
             raise RuntimeError(f"selective_scan: {name} must be {u.dtype} on {u.device} like u, got {t.dtype} on {t.device}")
-    delta, B, C, z = _adjacent(delta), _adjacent(B), _adjacent(C), _adjacent(z) if z is not None else None
-    A, D, delta_bias = (_float32("selective_scan", u, n, t, s)
-                        for n, t, s in (("A", A, (ch, N)), ("D", D, (ch,)), ("delta_bias", delta_bias, (ch,))))
-    state, state_out = _states("selective_scan", u, state, state_out, (nb, ch, N), torch.float32)
-    _no_grad("selective_scan", u, delta, z, B, C, A, D, delta_bias, state, state_out)
-    y = u.new_empty((nb, T, ch))
+    A = _float32("selective_scan", u, "A", A, (ch, N))
+    D = _float32("selective_scan", u, "D", D, (ch,))
+    delta_bias = _float32("selective_scan", u, "delta_bias", delta_bias, (ch,))
+    _states("selective_scan", u, state, state_out, (nb, ch, N), torch.float32)
+    if torch.is_grad_enabled():
+        _no_grad("selective_scan", u, delta, z, B, C, A, D, delta_bias, state, state_out)
+    y = torch.empty(shape, dtype=u.dtype, device=u.device)
     if nb and (T or state_out is not None):
         lengths = _lengths(lengths, nb, T, u)
+        delta, sd = _adjacent(delta)
+        z, sz = _adjacent(z) if z is not None else (None, (0, 0, 0))
+        B, sB = _adjacent(B)
+        C, sC = _adjacent(C)
+        f = len(shape) == 3  # with a frame axis
+        _call(_native.SELECTIVE_SCAN, u, T > 1, _native.SELECTIVE_SCAN.pack(
+            u.data_ptr(), sb, st, delta.data_ptr(), sd[0], sd[1] if f else 0, _ptr(z), sz[0], sz[1] if f else 0,
+            B.data_ptr(), sB[0], sB[1] if f else 0, C.data_ptr(), sC[0], sC[1] if f else 0, sB[-2] if G > 1 else 0,
+            sC[-2] if G > 1 else 0, y.data_ptr(), T * ch, ch, A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(state),
+            _ptr(state_out), _ptr(lengths), nb, T, ch, N, G, _DTYPES[u.dtype], 1 if delta_softplus else 0))
+    return y
 
-        def rows(t):
-            s = t.stride()
-            return t.data_ptr(), s[0], 0 if squeeze else s[1]
 
-        p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        a = _native.mv_selective_scan_args(
-            *rows(u), *rows(delta), *(rows(z) if z is not None else (None, 0, 0)), *rows(B), *rows(C),
-            B.stride(-2) if G > 1 else 0, C.stride(-2) if G > 1 else 0, y.data_ptr(), T * ch, ch, A.data_ptr(), p(D),
-            p(delta_bias), p(state), p(state_out), p(lengths), nb, T, ch, N, G, _DTYPES[u.dtype], 1 if delta_softplus else 0)
-        _call("mv_selective_scan", a, u, True)
-    return y[:, 0] if squeeze else y
+# --- arguments (checks are plain comparisons: a decode step's call is short against what Python adds to it) -----------
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
-# --- arguments -----------------------------------------------------------------------------------------------------
 def _adjacent(t):
-    """Channels side by side, other strides as they are."""
-    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+    """-> (t with channels side by side, its strides)"""
+    s = t.stride()
+    if s[-1] == 1 or t.shape[-1] == 1:
+        return t, s
+    t = t.contiguous()
+    return t, t.stride()
 
 
 def _data(who, name, x):
-    """-> (x with adjacent channels, B, T, channels, whether the frame axis is absent)"""
-    if x.dim() not in (2, 3) or x.size(-1) < 1:
-        raise RuntimeError(f"{who}: {name} must be [B, T, channels] or [B, channels], got {tuple(x.shape)}")
+    """-> (x with adjacent channels, its shape, B, T, channels, batch and row stride)"""
+    shape = x.shape
+    if len(shape) not in (2, 3) or shape[-1] < 1:
+        raise RuntimeError(f"{who}: {name} must be [B, T, channels] or [B, channels], got {tuple(shape)}")
     if not x.is_cuda:
         raise RuntimeError(f"tacotron2_amd.sequence.{who} computes on an MI355X only (no CPU fallback)")
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"{who}: {name} must be float32, bfloat16 or float16, got {x.dtype}")
-    x = _adjacent(x)
-    s = x.shape
-    return (x, s[0], s[1], s[2], False) if len(s) == 3 else (x, s[0], 1, s[1], True)
+    x, s = _adjacent(x)
+    if len(shape) == 3:
+        return x, shape, shape[0], shape[1], shape[2], s[0], s[1]
+    return x, shape, shape[0], 1, shape[1], s[0], 0
 
 
 def _activation(who, activation, slope):
@@ -180,40 +175,41 @@ def _activation(who, activation, slope):
     return _ACTIVATIONS[activation], 0.0 if activation == "relu" else float(slope)
 
 
-def _weights(who, x, named):
-    """Contiguous weights of one type: float32 or x's."""
-    out = []
-    for name, t, shape in named:
+def _weights(who, x, weight, shape, bias, ch):
+    """-> (weight, bias, MV_DTYPE_* of both): contiguous, of one type, float32 or x's."""
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        weight, bias = weight.float(), bias.float()
+    wtype = 0
+    for name, t, want in (("weight", weight, shape), ("bias", bias, (ch,))):
         if t is not None:
-            if tuple(t.shape) != shape or t.get_device() != x.get_device() or t.dtype not in (torch.float32, x.dtype):
-                raise RuntimeError(f"{who}: {name} must be {list(shape)}, float32 or {x.dtype}, on {x.device}; got "
+            if t.shape != want or t.get_device() != x.get_device() or not (t.dtype == torch.float32 or t.dtype == x.dtype):
+                raise RuntimeError(f"{who}: {name} must be {list(want)}, float32 or {x.dtype}, on {x.device}; got "
                                    f"{list(t.shape)}, {t.dtype}, on {t.device}")
-            t = t.contiguous()
-        out.append(t)
-    return out
+            wtype = _DTYPES[t.dtype]
+    return (weight if weight is None else weight.contiguous()), (bias if bias is None else bias.contiguous()), wtype
 
 
 def _float32(who, x, name, t, shape):
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.get_device() != x.get_device() or t.dtype not in _DTYPES:
+    if t.shape != shape or t.get_device() != x.get_device() or t.dtype not in _DTYPES:
         raise RuntimeError(f"{who}: {name} must be {list(shape)} floats on {x.device}, got {list(t.shape)}, {t.dtype}, on "
                            f"{t.device}")
-    return t.float().contiguous()
+    return t.contiguous() if t.dtype == torch.float32 else t.float().contiguous()
 
 
 def _states(who, x, state, state_out, shape, dtype):
     for name, t in (("state", state), ("state_out", state_out)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != x.get_device()
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != x.get_device()
                               or not t.is_contiguous()):
             raise RuntimeError(f"{who}: {name} must be contiguous {list(shape)}, {dtype}, on {x.device}; got "
                                f"{list(t.shape)}, {t.dtype}, on {t.device}")
-    return state, state_out
 
 
 def _no_grad(who, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"tacotron2_amd.sequence.{who} has no gradient: call it under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"tacotron2_amd.sequence.{who} has no gradient: call it under torch.no_grad()")
 
 
 def _lengths(lengths, B, T, x):
@@ -229,19 +225,22 @@ def _lengths(lengths, B, T, x):
     return _native.device_lengths(lengths, B, T, x.device)
 
 
-def _call(name, args, x, scratch):
-    """One call of the library on x's device and its current stream; scratch comes from torch's allocator (in a capture:
-    from the graph's own pool), a new piece for every call, so that no two calls or graphs share one."""
-    lib, dev = _native.lib(), x.get_device()
+def _call(op, x, scratch, args):
+    """One call of the library on x's device and its current stream.  Scratch (which calls of one frame do without) comes from
+    torch's allocator, in a capture from the graph's own pool: a new piece for every call, so that no two calls or graphs
+    share one."""
+    dev = x.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            return _call(name, args, x, scratch)
+            return _call(op, x, scratch, args)
+    if op.fn is None:
+        op.bind()
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    if scratch:
-        n = getattr(lib, name + "_workspace")(ctypes.byref(args))
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        rc = getattr(lib, name)(ctypes.byref(args), ws.data_ptr() if n else None, n, stream)
+    if not op.scratch:
+        rc = op.fn(args, stream)
     else:
-        rc = getattr(lib, name)(ctypes.byref(args), stream)
+        n = op.fn_workspace(args) if scratch else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        rc = op.fn(args, _ptr(ws), n, stream)
     if rc:
-        _native.check(rc, name)
+        _native.check(rc, op.name)
