@@ -20,26 +20,6 @@ struct CausalParams {
     int vecs, run, runs;  // vectors of a row, frames a thread walks, threads to a sequence's vector
 };
 
-// V channels at p, or the first `n` of them
-template <typename T, int V>
-__device__ __forceinline__ typename Unaligned<T, V>::type load_some(const T* p, int n) {
-    typename Unaligned<T, V>::type v;
-    if (n == V) return *(const typename Unaligned<T, V>::type*)p;
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = e < n ? p[e] : (T)0.f;
-    return v;
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_some(T* p, typename Unaligned<T, V>::type v, int n) {
-    if (n == V) {
-        *(typename Unaligned<T, V>::type*)p = v;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (e < n) p[e] = v[e];
-}
-
 constexpr int kConvStep = 4;  // frames whose loads are in flight together
 
 // A thread walks `run` frames of V adjacent channels with the K - 1 frames before in registers.  The thread of a sequence's

@@ -21,8 +21,18 @@ __device__ __forceinline__ float softplusf(float x) {
 }
 
 constexpr int kLanes = 4;   // lanes that share a channel: lane 4c + j holds states j * NS ... of channel c
-constexpr int kTile = 32;   // frames whose B and C rows are in LDS at a time
 constexpr int kBlockChannels = 64;  // 4 waves of 16 channels
+
+// A tile of frames in LDS: u, delta, z as they are stored, rows of 64 channels padded so that the four rows that a wave reads
+// at once (4 lanes a channel, each on a frame of its own) lie in different banks; B and C as float32 [frame][4 * NS].
+template <typename T, int NS>
+struct Tile {
+    static constexpr int frames = 64 / (int)sizeof(T), NP = kLanes * NS;
+    static constexpr int vec = 16 / (int)sizeof(T), vecs = kBlockChannels / vec;  // vectors of a row
+    static constexpr int row = kBlockChannels + 16;                                // elements
+    T rows[3][frames][row];
+    float maps[2][frames][NP];
+};
 
 template <typename T>
 struct ScanParams {
@@ -34,16 +44,16 @@ struct ScanParams {
     long long Bg, Cg;
     float *ws_h, *ws_s;  // pieces' states from zero [B][pieces - 1][D][4 * NS] and sums of dt [B][pieces - 1][D]
     int B, Tmax, D, N, G, softplus;
-    int blocks_per_group, piece, pieces;  // frames to a piece (a multiple of kTile), number of pieces
+    int blocks_per_group, piece, pieces;  // frames to a piece (a multiple of 32), number of pieces
 };
 
 template <int CTRL>
 __device__ __forceinline__ float quad(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-template <int K>
-__device__ __forceinline__ float quad_lane(float v) {
-    return quad<K * 0x55>(v);
+// lane k's value in all four (k is a constant once the loop around it is unrolled)
+__device__ __forceinline__ float quad_lane(float v, int k) {
+    return k == 0 ? quad<0x00>(v) : k == 1 ? quad<0x55>(v) : k == 2 ? quad<0xAA>(v) : quad<0xFF>(v);
 }
 
 // Lane j's NS of the N values at p, as floats; zeros where it has fewer.
@@ -119,96 +129,91 @@ __device__ __forceinline__ void load_states(const float* p, float (&v)[NS]) {
     }
 }
 
-// One of u, delta, z, y as a channel block walks it: 16 frames at a time, lane j of a channel on frames j, j + 4, j + 8, j + 12
-// of them.  The address of a frame is a base that all lanes share (scalar arithmetic) plus an offset that a lane keeps.
-template <typename T>
-struct Walk {
-    T* p;             // channel 0 of frame 0 of the sequence
-    long long rs;
-    unsigned lane;    // bytes
-    __device__ __forceinline__ Walk(const Rows<T>& r, int b, int d, int j)
-        : p(r.p ? r.row(b, 0) : nullptr), rs(r.rs), lane((unsigned)(j * r.rs + d) * (unsigned)sizeof(T)) {}
-    __device__ __forceinline__ T* at(int t, int i) const { return (T*)((char*)(p + (t + 4 * i) * rs) + lane); }
-    // the same with frames from `end` on replaced by frame end - 1
-    __device__ __forceinline__ T* at_or_last(int t, int i, int end, int j) const {
-        const int r = min(4 * i + j, end - 1 - t) - j;
-        return (T*)((char*)(p + t * rs) + (long long)(r * (int)rs) * (int)sizeof(T) + lane);
-    }
-};
-
 // Frames [t0, t1) of one channel block: h goes from the state before t0 to the state after t1 - 1.  Y: results are stored;
 // otherwise only the states move, and the sum of dt is returned.
 template <typename T, int NS, bool Y>
-__device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Channel<T, NS>& ch, int t0, int t1, float (&h)[NS],
-                                             float* lds) {
-    constexpr int NP = kLanes * NS, kMine = kTile * NP / 256 > 0 ? kTile * NP / 256 : 1;
+__device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Channel<T, NS>& ch, int c0, int t0, int t1,
+                                             float (&h)[NS], Tile<T, NS>* lds) {
+    typedef Tile<T, NS> Tl;
+    typedef typename Unaligned<T, Tl::vec>::type Vec;
+    constexpr int NP = Tl::NP, kMine = Tl::frames * NP / 256 > 0 ? Tl::frames * NP / 256 : 1;
     const int tid = threadIdx.x;
     const float bias = p.bias ? p.bias[ch.d] : 0.f, skip = p.Dskip ? p.Dskip[ch.d] : 0.f;
-    const Walk<const T> uw(p.u, ch.b, ch.d, ch.j), dw(p.delta, ch.b, ch.d, ch.j), zw(p.z, ch.b, ch.d, ch.j);
-    const Walk<T> yw(p.y, ch.b, ch.d, ch.j);
-    const T* Bb = p.Bm.row(ch.b, 0) + ch.g * p.Bg;
-    const T* Cb = p.Cm.row(ch.b, 0) + ch.g * p.Cg;
+    const bool gate = Y && p.z.p;
     float sum = 0.f;
 
-    // B and C rows of the next tile on their way to LDS, u, delta and z of the next 16 frames on their way to the lanes;
-    // a frame past t1 reads frame t1 - 1 and is replaced by zeros, which leave the state as it is (dt = 0)
-    T nb[kMine], nc[kMine], nu[4], nd[4], nz[4];
-    auto fetch_maps = [&](int t) {
+    // The next tile on its way: a thread brings one vector of a row of u, delta, z each (256 threads cover a tile) and kMine
+    // elements of B and C.  A frame past t1 - 1 is that frame again; nothing reads it but for zeros in its place.  Addresses
+    // are a base that all threads share (scalar arithmetic) plus an offset that a thread keeps.
+    const int vrow = tid / Tl::vecs, vcol = tid % Tl::vecs * Tl::vec;
+    const int vn = min(Tl::vec, p.D / p.G - c0 - vcol);  // channels of the vector that the group has
+    const int d0 = ch.g * (p.D / p.G) + c0 + vcol;
+    constexpr int kRows = 256 / NP > Tl::frames ? Tl::frames : 256 / NP;  // rows of B and C that the block brings at once
+    const int mrow = tid / NP % Tl::frames, mn = min(tid % NP, p.N - 1);
+    const long long Bg = ch.g * p.Bg, Cg = ch.g * p.Cg;
+    Vec nv[3];
+    T nb[kMine], nc[kMine];
+    auto at = [&](const Rows<const T>& r, long long off, int t, int row, int col) {
+        const T* base = r.row(ch.b, t) + off;
+        return (const T*)((const char*)base + (unsigned)(row * (int)r.rs + col) * (unsigned)sizeof(T));
+    };
+    auto fetch = [&](int t) {
+        const int last = t1 - 1 - t;
+        const int r = min(vrow, last);
+        if (vn > 0) {
+            nv[0] = load_some<T, Tl::vec>(at(p.u, 0, t, r, d0), vn);
+            nv[1] = load_some<T, Tl::vec>(at(p.delta, 0, t, r, d0), vn);
+            if (gate) nv[2] = load_some<T, Tl::vec>(at(p.z, 0, t, r, d0), vn);
+        }
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-            const int e = tid + 256 * i, n = min(e % NP, p.N - 1);
-            const long long r = min(t + e / NP % kTile, t1 - 1);
-            nb[i] = Bb[r * p.Bm.rs + n];
-            if (Y) nc[i] = Cb[r * p.Cm.rs + n];
+            const int m = min(mrow + i * kRows, last);
+            nb[i] = *at(p.Bm, Bg, t, m, mn);
+            if (Y) nc[i] = *at(p.Cm, Cg, t, m, mn);
         }
     };
-    auto put_maps = [&](int t, float* to) {
+    auto put = [&](int t, Tl& to) {
+        *(Vec*)&to.rows[0][vrow][vcol] = nv[0];
+        *(Vec*)&to.rows[1][vrow][vcol] = nv[1];
+        if (gate) *(Vec*)&to.rows[2][vrow][vcol] = nv[2];
+        const bool whole = p.N == NP && t + Tl::frames <= t1;
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int e = tid + 256 * i;
-            const bool in = e % NP < p.N && t + e / NP < t1;
-            if (e < kTile * NP) {
-                to[e] = in ? (float)nb[i] : 0.f;
-                if (Y) to[kTile * NP + e] = in ? (float)nc[i] : 0.f;
+            float vb = (float)nb[i], vc = Y ? (float)nc[i] : 0.f;
+            if (!whole && !(e % NP < p.N && t + e / NP < t1)) vb = vc = 0.f;
+            if (256 * (i + 1) <= Tl::frames * NP || e < Tl::frames * NP) {
+                to.maps[0][0][e] = vb;
+                if (Y) to.maps[1][0][e] = vc;
             }
         }
     };
-    auto fetch_frames = [&](int t) {
-        const bool whole = t + 16 <= t1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            nu[i] = *(whole ? uw.at(t, i) : uw.at_or_last(t, i, t1, ch.j));
-            nd[i] = *(whole ? dw.at(t, i) : dw.at_or_last(t, i, t1, ch.j));
-        }
-        if (Y && zw.p) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) nz[i] = *(whole ? zw.at(t, i) : zw.at_or_last(t, i, t1, ch.j));
-        }
-    };
-    fetch_maps(t0);
-    fetch_frames(t0);
+    const int cl = tid >> 2;                      // the lane's channel of the block's 64
+    const int lane = tid & 63, wave = tid >> 6;   // results leave 16 bytes a lane: 16 channels of a frame on two or four lanes
+    constexpr int kOut = 16 / Tl::vec, kOutRows = 64 / kOut;
+    const int orow = lane / kOut, ocol = wave * 16 + lane % kOut * Tl::vec;
+    const int on = min(Tl::vec, p.D / p.G - c0 - ocol);
+    fetch(t0);
     int buf = 0;
-    for (int t = t0; t < t1; t += kTile, buf ^= 1) {
-        float* maps = lds + buf * 2 * kTile * NP;
-        put_maps(t, maps);
+    for (int t = t0; t < t1; t += Tl::frames, buf ^= 1) {
+        Tl& tile = lds[buf];
+        put(t, tile);
         __syncthreads();
-        if (t + kTile < t1) fetch_maps(t + kTile);
+        if (t + Tl::frames < t1) fetch(t + Tl::frames);
 #pragma unroll 1
-        for (int q = 0; q < kTile && t + q < t1; q += 16) {
-            const bool whole = t + q + 16 <= t1;
+        for (int q = 0; q < Tl::frames && t + q < t1; q += 16) {
             float uv[4], dv[4], xv[4], zv[4], yv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uv[i] = (float)nu[i];
-                dv[i] = (float)nd[i] + bias;
-                if (Y && zw.p) zv[i] = (float)nz[i];
+                uv[i] = (float)tile.rows[0][q + 4 * i + ch.j][cl];
+                dv[i] = (float)tile.rows[1][q + 4 * i + ch.j][cl] + bias;
+                if (gate) zv[i] = (float)tile.rows[2][q + 4 * i + ch.j][cl];
             }
-            if (t + q + 16 < t1) fetch_frames(t + q + 16);
             if (p.softplus) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dv[i] = softplusf(dv[i]);
             }
-            if (!whole) {
+            if (t + q + 16 > t1) {  // frames past the end leave the state as it is: dt = 0
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (t + q + 4 * i + ch.j >= t1) uv[i] = dv[i] = 0.f;
@@ -218,46 +223,70 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
                 xv[i] = dv[i] * uv[i];
                 if (!Y) sum += dv[i];
             }
+            // F frames at a time: their decays first, 16 exponentials that depend on nothing, then the chain through h; the
+            // B and C values of the next F frames come out of LDS meanwhile
+            constexpr int F = NS >= 16 ? 1 : NS == 8 ? 2 : 4;
+            float bn[2][F][NS], cn[2][F][NS], out[4];
+            auto read = [&](int unit, int to) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float out[4];
-                auto frame = [&](auto k) {
-                    constexpr int K = decltype(k)::value;
-                    const float dt = quad_lane<K>(dv[i]), x = quad_lane<K>(xv[i]);
-                    const float* row = maps + (q + 4 * i + K) * NP + ch.j * NS;
-                    float bn[NS], cn[NS], o = 0.f;
-                    load_states<NS>(row, bn);
-                    if (Y) load_states<NS>(row + kTile * NP, cn);
+                for (int f = 0; f < F; ++f) {
+                    load_states<NS>(&tile.maps[0][q + unit * F + f][ch.j * NS], bn[to][f]);
+                    if (Y) load_states<NS>(&tile.maps[1][q + unit * F + f][ch.j * NS], cn[to][f]);
+                }
+            };
+            read(0, 0);
+#pragma unroll
+            for (int unit = 0; unit < 16 / F; ++unit) {
+                const int now = unit & 1;
+                if (unit + 1 < 16 / F) read(unit + 1, now ^ 1);
+                float decay[F][NS], x[F];
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    const int k = unit * F + f;
+                    const float dt = quad_lane(dv[k / 4], k % 4);
+                    x[f] = quad_lane(xv[k / 4], k % 4);
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) decay[f][s] = __builtin_amdgcn_exp2f(dt * ch.A2[s]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    float o = 0.f;
 #pragma unroll
                     for (int s = 0; s < NS; ++s) {
-                        h[s] = __builtin_amdgcn_exp2f(dt * ch.A2[s]) * h[s] + x * bn[s];
-                        if (Y) o = s ? o + cn[s] * h[s] : cn[s] * h[s];
+                        h[s] = decay[f][s] * h[s] + x[f] * bn[now][f][s];
+                        if (Y) o = s ? o + cn[now][f][s] * h[s] : cn[now][f][s] * h[s];
                     }
-                    out[K] = o;
-                };
-                frame(std::integral_constant<int, 0>());
-                frame(std::integral_constant<int, 1>());
-                frame(std::integral_constant<int, 2>());
-                frame(std::integral_constant<int, 3>());
-                if (Y) {
+                    out[(unit * F + f) % 4] = o;
+                }
+                if (Y && (unit * F + F) % 4 == 0) {
                     // out[k] of the four lanes added up, frame k's sum to lane k
+                    const int i = (unit * F) / 4;
                     const bool o1 = ch.j & 1, o2 = ch.j & 2;
                     const float a = (o1 ? out[1] : out[0]) + quad<0xB1>(o1 ? out[0] : out[1]);
                     const float b = (o1 ? out[3] : out[2]) + quad<0xB1>(o1 ? out[2] : out[3]);
                     yv[i] = (o2 ? b : a) + quad<0x4E>(o2 ? a : b) + skip * uv[i];
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (Y) {
-                if (zw.p) {
+                if (gate) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) yv[i] *= zv[i] * sigmoidf(zv[i]);
                 }
-                if (ch.live) {
+                // the results take the place of the u that they came from (the same lane's, read above)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (whole || t + q + 4 * i + ch.j < t1) *yw.at(t + q, i) = (T)yv[i];
-                }
+                for (int i = 0; i < 4; ++i) tile.rows[0][q + 4 * i + ch.j][cl] = (T)yv[i];
             }
+        }
+        if (Y) {
+            // a wave reads back what its own lanes wrote: LDS serves a wave's operations in their order
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = orow; r < Tl::frames; r += kOutRows)
+                if (on > 0 && t + r < t1)
+                    store_some<T, Tl::vec>(p.y.row(ch.b, t + r) + ch.g * (p.D / p.G) + c0 + ocol, *(const Vec*)&tile.rows[0][r][ocol], on);
         }
         // (the next tile goes to the other buffer; the one after it comes behind the next barrier)
     }
@@ -287,12 +316,13 @@ __device__ __forceinline__ float* piece_sum(const ScanParams<T>& p, const Channe
 // state before it, which it puts together from what the first launch left.
 template <typename T, int NS, bool FIRST>
 __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
-    __shared__ float lds[2 * 2 * kTile * kLanes * NS];
+    __shared__ Tile<T, NS> lds[2];
     Channel<T, NS> ch;
     const int g = blockIdx.x / p.blocks_per_group, cb = blockIdx.x % p.blocks_per_group;
     const int piece = FIRST ? blockIdx.y : blockIdx.y + 1;
     for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
-        ch.init(p, b, g, cb * kBlockChannels + (threadIdx.x >> 2));
+        const int c0 = cb * kBlockChannels;
+        ch.init(p, b, g, c0 + (threadIdx.x >> 2));
         const long long first = (long long)piece * p.piece;
         const int t0 = (int)min(first, (long long)p.Tmax), te = (int)min(first + p.piece, (long long)p.Tmax);
         const int t1 = min(te, ch.len);
@@ -302,7 +332,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             if (!last) {
 #pragma unroll
                 for (int s = 0; s < NS; ++s) h[s] = 0.f;
-                const float sum = scan_frames<T, NS, false>(p, ch, t0, t1, h, lds);
+                const float sum = scan_frames<T, NS, false>(p, ch, c0, t0, t1, h, lds);
                 if (ch.live) {
                     float* to = piece_states(p, ch, piece);
 #pragma unroll
@@ -317,14 +347,23 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
                 const float* from = piece_states(p, ch, 0);
 #pragma unroll
                 for (int s = 0; s < NS; ++s) h[s] = from[s];
-                for (int k = 1; k < piece; ++k) {
-                    from = piece_states(p, ch, k);
-                    const float sum = *piece_sum(p, ch, k);
+                constexpr int kBatch = NS >= 16 ? 2 : 8;  // pieces whose loads are in flight together
+                for (int k = 1; k < piece; k += kBatch) {
+                    float sum[kBatch], end[kBatch][NS];
 #pragma unroll
-                    for (int s = 0; s < NS; ++s) h[s] = __builtin_amdgcn_exp2f(sum * ch.A2[s]) * h[s] + from[s];
+                    for (int i = 0; i < kBatch; ++i) {
+                        const int at = min(k + i, piece - 1);
+                        load_states<NS>(piece_states(p, ch, at), end[i]);
+                        sum[i] = *piece_sum(p, ch, at);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i)
+                        if (k + i < piece)
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) h[s] = __builtin_amdgcn_exp2f(sum[i] * ch.A2[s]) * h[s] + end[i][s];
                 }
             }
-            if (t0 < t1) scan_frames<T, NS, true>(p, ch, t0, t1, h, lds);
+            if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds);
             if (last) {
                 ch.store_state(p, h);
             } else if (FIRST && ch.live) {
@@ -398,7 +437,7 @@ static ScanPlan scan_plan(const mv_selective_scan_args* a) {
     s.NS = 1;
     while (s.NS * kLanes < a->N) s.NS *= 2;
     s.pieces = a->T <= kStepFrames ? 1 : scan_pieces(a->B, a->T, a->D, a->G);
-    s.piece = round_up((a->T + s.pieces - 1) / s.pieces, kTile);
+    s.piece = round_up((a->T + s.pieces - 1) / s.pieces, 32);
     s.pieces = (int)(((long long)a->T + s.piece - 1) / s.piece);
     if (s.pieces > 1) {
         const size_t n = (size_t)a->B * (s.pieces - 1) * a->D;

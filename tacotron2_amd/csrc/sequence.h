@@ -24,6 +24,26 @@ struct Unaligned {
     typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
+// V channels at p, or the first `n` of them
+template <typename T, int V>
+__device__ __forceinline__ typename Unaligned<T, V>::type load_some(const T* p, int n) {
+    typename Unaligned<T, V>::type v;
+    if (n == V) return *(const typename Unaligned<T, V>::type*)p;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < n ? p[e] : (T)0.f;
+    return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T* p, typename Unaligned<T, V>::type v, int n) {
+    if (n == V) {
+        *(typename Unaligned<T, V>::type*)p = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < n) p[e] = v[e];
+}
+
 constexpr float kLog2e = 1.44269504088896341f;
 
 // sigmoid and its relatives on the hardware exp2 and reciprocal (1 ulp each): exp2 overflowing to inf gives the right 0
