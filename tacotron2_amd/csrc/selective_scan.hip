@@ -20,11 +20,21 @@ __device__ __forceinline__ float softplusf(float x) {
     return fmaxf(x, 0.f) + 2.f * s * (p * q + 1.f);
 }
 
-constexpr int kLanes = 4;   // lanes that share a channel: lane 4c + j holds states j * NS ... of channel c
+// Four lanes share a channel; lane j of them holds states `state_of(j, 0 ... NS - 1)`: runs of four that a 16 x 16 outer
+// product leaves in a lane (below), or of NS where a channel has fewer than 16.
+constexpr int kLanes = 4;
+template <int NS>
+__device__ __forceinline__ constexpr int state_of(int j, int s) {
+    return NS >= 4 ? 16 * (s / 4) + 4 * j + s % 4 : NS * j + s;
+}
+template <int NS>
+constexpr int kRun = NS >= 4 ? 4 : NS;  // adjacent states of a lane
+
 constexpr int kBlockChannels = 64;  // 4 waves of 16 channels
 
 // A tile of frames in LDS: u, delta, z as they are stored, rows of 64 channels padded so that the four rows that a wave reads
-// at once (4 lanes a channel, each on a frame of its own) lie in different banks; B and C as float32 [frame][4 * NS].
+// at once (lane 16 j + c is on channel c of a frame of its own) lie in different banks; B and C as float32 [frame][4 * NS];
+// the steps dt of 16 frames by channel, each wave's own.
 template <typename T, int NS>
 struct Tile {
     static constexpr int frames = 64 / (int)sizeof(T), NP = kLanes * NS;
@@ -33,6 +43,7 @@ struct Tile {
     T rows[3][frames][row];
     float maps[2][frames][NP];
 };
+constexpr int kStepRow = 20;  // floats: 16 frames, padded
 
 template <typename T>
 struct ScanParams {
@@ -51,22 +62,38 @@ template <int CTRL>
 __device__ __forceinline__ float quad(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-// lane k's value in all four (k is a constant once the loop around it is unrolled)
-__device__ __forceinline__ float quad_lane(float v, int k) {
-    return k == 0 ? quad<0x00>(v) : k == 1 ? quad<0x55>(v) : k == 2 ? quad<0xAA>(v) : quad<0xFF>(v);
-}
 
 // Lane j's NS of the N values at p, as floats; zeros where it has fewer.
 template <typename T, int NS>
 __device__ __forceinline__ void load_my_states(const T* p, int N, int j, float (&v)[NS]) {
     if (N == kLanes * NS) {
-        typedef typename Unaligned<T, NS>::type V;
-        const V t = *(const V*)(p + j * NS);
+        typedef typename Unaligned<T, kRun<NS>>::type V;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) v[s] = (float)t[s];
+        for (int s = 0; s < NS; s += kRun<NS>) {
+            const V t = *(const V*)(p + state_of<NS>(j, s));
+#pragma unroll
+            for (int e = 0; e < kRun<NS>; ++e) v[s + e] = (float)t[e];
+        }
     } else {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) v[s] = j * NS + s < N ? (float)p[j * NS + s] : 0.f;
+        for (int s = 0; s < NS; ++s) v[s] = state_of<NS>(j, s) < N ? (float)p[state_of<NS>(j, s)] : 0.f;
+    }
+}
+template <int NS>
+__device__ __forceinline__ void store_my_states(float* p, int N, int j, const float (&v)[NS]) {
+    if (N == kLanes * NS) {
+        typedef typename Unaligned<float, kRun<NS>>::type V;
+#pragma unroll
+        for (int s = 0; s < NS; s += kRun<NS>) {
+            V t;
+#pragma unroll
+            for (int e = 0; e < kRun<NS>; ++e) t[e] = v[s + e];
+            *(V*)(p + state_of<NS>(j, s)) = t;
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+            if (state_of<NS>(j, s) < N) p[state_of<NS>(j, s)] = v[s];
     }
 }
 
@@ -77,9 +104,9 @@ struct Channel {
     bool live;   // false: a lane past the group's last channel, which computes on the last one and stores nothing
     float A2[NS];
 
-    __device__ __forceinline__ void init(const ScanParams<T>& p, int b_, int g_, int c) {
+    __device__ __forceinline__ void init(const ScanParams<T>& p, int b_, int g_, int c, int j_) {
         const int Dg = p.D / p.G;
-        b = b_, g = g_, j = threadIdx.x & (kLanes - 1);
+        b = b_, g = g_, j = j_;
         live = c < Dg;
         d = g * Dg + min(c, Dg - 1);
         len = seq_frames(p.lengths, b, p.Tmax);
@@ -100,32 +127,32 @@ struct Channel {
         }
     }
     __device__ __forceinline__ void store_state(const ScanParams<T>& p, const float (&h)[NS]) const {
-        if (!p.state_out || !live) return;
-        float* to = p.state_out + ((long long)b * p.D + d) * p.N;
-        if (p.N == kLanes * NS) {
-            typedef typename Unaligned<float, NS>::type V;
-            V v;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) v[s] = h[s];
-            *(V*)(to + j * NS) = v;
-        } else {
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                if (j * NS + s < p.N) to[j * NS + s] = h[s];
-        }
+        if (p.state_out && live) store_my_states(p.state_out + ((long long)b * p.D + d) * p.N, p.N, j, h);
     }
 };
 
+// a[k] of four values, each spread over the four rows of 16 lanes: row k gets the sum of a[k]
+__device__ __forceinline__ float sum_rows(const float (&a)[4]) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    auto both = [](u32x2 v) {
+        const unsigned x = v[0], y = v[1];
+        return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+    };
+    auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+    const float lo = both(__builtin_amdgcn_permlane16_swap(bits(a[0]), bits(a[1]), false, false));
+    const float hi = both(__builtin_amdgcn_permlane16_swap(bits(a[2]), bits(a[3]), false, false));
+    return both(__builtin_amdgcn_permlane32_swap(bits(lo), bits(hi), false, false));
+}
+
+// lane j's states of a row of 4 * NS floats in LDS
 template <int NS>
-__device__ __forceinline__ void load_states(const float* p, float (&v)[NS]) {
-    if constexpr (NS % 4 == 0) {
+__device__ __forceinline__ void load_lane_states(const float* row, int j, float (&v)[NS]) {
+    typedef float V __attribute__((ext_vector_type(kRun<NS>)));
 #pragma unroll
-        for (int s = 0; s < NS; s += 4) *(f32x4*)&v[s] = *(const f32x4*)&p[s];
-    } else if constexpr (NS == 2) {
-        const float2 t = *(const float2*)p;
-        v[0] = t.x, v[1] = t.y;
-    } else {
-        v[0] = p[0];
+    for (int s = 0; s < NS; s += kRun<NS>) {
+        const V t = *(const V*)&row[state_of<NS>(j, s)];
+#pragma unroll
+        for (int e = 0; e < kRun<NS>; ++e) v[s + e] = t[e];
     }
 }
 
@@ -133,7 +160,7 @@ __device__ __forceinline__ void load_states(const float* p, float (&v)[NS]) {
 // otherwise only the states move, and the sum of dt is returned.
 template <typename T, int NS, bool Y>
 __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Channel<T, NS>& ch, int c0, int t0, int t1,
-                                             float (&h)[NS], Tile<T, NS>* lds) {
+                                             float (&h)[NS], Tile<T, NS>* lds, float* steps) {
     typedef Tile<T, NS> Tl;
     typedef typename Unaligned<T, Tl::vec>::type Vec;
     constexpr int NP = Tl::NP, kMine = Tl::frames * NP / 256 > 0 ? Tl::frames * NP / 256 : 1;
@@ -188,8 +215,9 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
             }
         }
     };
-    const int cl = tid >> 2;                      // the lane's channel of the block's 64
-    const int lane = tid & 63, wave = tid >> 6;   // results leave 16 bytes a lane: 16 channels of a frame on two or four lanes
+    const int lane = tid & 63, wave = tid >> 6, cl = wave * 16 + (lane & 15);  // the lane's channel of the block's 64
+    float* mine = steps + cl * kStepRow;
+    // results leave 16 bytes a lane: 16 channels of a frame on two or four lanes
     constexpr int kOut = 16 / Tl::vec, kOutRows = 64 / kOut;
     const int orow = lane / kOut, ocol = wave * 16 + lane % kOut * Tl::vec;
     const int on = min(Tl::vec, p.D / p.G - c0 - ocol);
@@ -223,49 +251,76 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
                 xv[i] = dv[i] * uv[i];
                 if (!Y) sum += dv[i];
             }
-            // F frames at a time: their decays first, 16 exponentials that depend on nothing, then the chain through h; the
-            // B and C values of the next F frames come out of LDS meanwhile
+            // A lane has the steps of the frames that it loaded; all four lanes of a channel need each of them
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mine[4 * i + ch.j] = dv[i];
+                if (NS < 4) mine[64 * kStepRow + 4 * i + ch.j] = xv[i];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // F frames at a time: their decays first, exponentials that depend on nothing, then the chain through h; C values
+            // come out of LDS meanwhile.  dt u B of four frames is four outer products, 16 channels by 16 states, on the
+            // matrix unit beside the vector unit's exponentials.
             constexpr int F = NS >= 16 ? 1 : NS == 8 ? 2 : 4;
-            float bn[2][F][NS], cn[2][F][NS], out[4];
+            float cn[2][F][NS], out[4];
             auto read = [&](int unit, int to) {
 #pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    load_states<NS>(&tile.maps[0][q + unit * F + f][ch.j * NS], bn[to][f]);
-                    if (Y) load_states<NS>(&tile.maps[1][q + unit * F + f][ch.j * NS], cn[to][f]);
-                }
+                for (int f = 0; f < F; ++f)
+                    load_lane_states<NS>(tile.maps[1][q + unit * F + f], ch.j, cn[to][f]);
             };
-            read(0, 0);
+            if (Y) read(0, 0);
+            f32x4 xb[4][NS >= 4 ? NS / 4 : 1];
+            float dt4[4];
 #pragma unroll
             for (int unit = 0; unit < 16 / F; ++unit) {
                 const int now = unit & 1;
-                if (unit + 1 < 16 / F) read(unit + 1, now ^ 1);
-                float decay[F][NS], x[F];
+                if (Y && unit + 1 < 16 / F) read(unit + 1, now ^ 1);
+                if (unit * F % 4 == 0) {
+                    const int i = unit * F / 4;
+                    const f32x4 d4 = *(const f32x4*)&mine[4 * i];
 #pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    const int k = unit * F + f;
-                    const float dt = quad_lane(dv[k / 4], k % 4);
-                    x[f] = quad_lane(xv[k / 4], k % 4);
+                    for (int k = 0; k < 4; ++k) dt4[k] = d4[k];
+                    if constexpr (NS >= 4) {
 #pragma unroll
-                    for (int s = 0; s < NS; ++s) decay[f][s] = __builtin_amdgcn_exp2f(dt * ch.A2[s]);
+                        for (int m = 0; m < NS / 4; ++m) {
+                            typedef float f32x16 __attribute__((ext_vector_type(16)));
+                            const float bn = tile.maps[0][q + 4 * i + ch.j][16 * m + (lane & 15)];
+                            const f32x16 v = __builtin_amdgcn_mfma_f32_16x16x1f32(bn, xv[i], f32x16{}, 0, 0, 0);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) xb[k][m] = f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                        }
+                    } else {
+                        const f32x4 x4 = *(const f32x4*)&mine[64 * kStepRow + 4 * i];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float bn[NS];
+                            load_lane_states<NS>(tile.maps[0][q + 4 * i + k], ch.j, bn);
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) xb[k][0][s] = x4[k] * bn[s];
+                        }
+                    }
                 }
+                float decay[F][NS];
+#pragma unroll
+                for (int f = 0; f < F; ++f)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) decay[f][s] = __builtin_amdgcn_exp2f(dt4[(unit * F + f) % 4] * ch.A2[s]);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int f = 0; f < F; ++f) {
+                    const int k = (unit * F + f) % 4;
                     float o = 0.f;
 #pragma unroll
                     for (int s = 0; s < NS; ++s) {
-                        h[s] = decay[f][s] * h[s] + x[f] * bn[now][f][s];
-                        if (Y) o = s ? o + cn[now][f][s] * h[s] : cn[now][f][s] * h[s];
+                        h[s] = __builtin_fmaf(decay[f][s], h[s], xb[k][s / 4][s % 4]);
+                        if (Y) o = s ? __builtin_fmaf(cn[now][f][s], h[s], o) : cn[now][f][s] * h[s];
                     }
-                    out[(unit * F + f) % 4] = o;
+                    out[k] = o;
                 }
                 if (Y && (unit * F + F) % 4 == 0) {
-                    // out[k] of the four lanes added up, frame k's sum to lane k
                     const int i = (unit * F) / 4;
-                    const bool o1 = ch.j & 1, o2 = ch.j & 2;
-                    const float a = (o1 ? out[1] : out[0]) + quad<0xB1>(o1 ? out[0] : out[1]);
-                    const float b = (o1 ? out[3] : out[2]) + quad<0xB1>(o1 ? out[2] : out[3]);
-                    yv[i] = (o2 ? b : a) + quad<0x4E>(o2 ? a : b) + skip * uv[i];
+                    yv[i] = sum_rows(out) + skip * uv[i];
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -290,7 +345,7 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         }
         // (the next tile goes to the other buffer; the one after it comes behind the next barrier)
     }
-    if (!Y) sum += quad<0xB1>(sum), sum += quad<0x4E>(sum);
+    if (!Y) sum += __shfl_xor(sum, 16), sum += __shfl_xor(sum, 32);
     return sum;
 }
 
@@ -302,9 +357,10 @@ __device__ __forceinline__ void zero_frames(const ScanParams<T>& p, const Channe
         for (int t = t0 + ch.j; t < t1; t += kLanes) yb[(long long)t * p.y.rs] = (T)0.f;
 }
 
+// (4 * NS floats)
 template <typename T, int NS>
 __device__ __forceinline__ float* piece_states(const ScanParams<T>& p, const Channel<T, NS>& ch, int piece) {
-    return p.ws_h + (((long long)ch.b * (p.pieces - 1) + piece) * p.D + ch.d) * (kLanes * NS) + ch.j * NS;
+    return p.ws_h + (((long long)ch.b * (p.pieces - 1) + piece) * p.D + ch.d) * (kLanes * NS);
 }
 template <typename T, int NS>
 __device__ __forceinline__ float* piece_sum(const ScanParams<T>& p, const Channel<T, NS>& ch, int piece) {
@@ -316,13 +372,14 @@ __device__ __forceinline__ float* piece_sum(const ScanParams<T>& p, const Channe
 // state before it, which it puts together from what the first launch left.
 template <typename T, int NS, bool FIRST>
 __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
-    __shared__ Tile<T, NS> lds[2];
+    __shared__ __align__(16) Tile<T, NS> lds[2];
+    __shared__ __align__(16) float steps[(NS < 4 ? 2 : 1) * kBlockChannels * kStepRow];
     Channel<T, NS> ch;
     const int g = blockIdx.x / p.blocks_per_group, cb = blockIdx.x % p.blocks_per_group;
     const int piece = FIRST ? blockIdx.y : blockIdx.y + 1;
     for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
         const int c0 = cb * kBlockChannels;
-        ch.init(p, b, g, c0 + (threadIdx.x >> 2));
+        ch.init(p, b, g, c0 + threadIdx.x / 64 * 16 + threadIdx.x % 16, threadIdx.x % 64 / 16);
         const long long first = (long long)piece * p.piece;
         const int t0 = (int)min(first, (long long)p.Tmax), te = (int)min(first + p.piece, (long long)p.Tmax);
         const int t1 = min(te, ch.len);
@@ -332,11 +389,9 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             if (!last) {
 #pragma unroll
                 for (int s = 0; s < NS; ++s) h[s] = 0.f;
-                const float sum = scan_frames<T, NS, false>(p, ch, c0, t0, t1, h, lds);
+                const float sum = scan_frames<T, NS, false>(p, ch, c0, t0, t1, h, lds, steps);
                 if (ch.live) {
-                    float* to = piece_states(p, ch, piece);
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) to[s] = h[s];
+                    store_my_states(piece_states(p, ch, piece), kLanes * NS, ch.j, h);
                     if (ch.j == 0) *piece_sum(p, ch, piece) = sum;
                 }
             }
@@ -344,16 +399,14 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             if (FIRST) {
                 ch.load_state(p, h);
             } else {
-                const float* from = piece_states(p, ch, 0);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) h[s] = from[s];
+                load_my_states(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
                 constexpr int kBatch = NS >= 16 ? 2 : 8;  // pieces whose loads are in flight together
                 for (int k = 1; k < piece; k += kBatch) {
                     float sum[kBatch], end[kBatch][NS];
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         const int at = min(k + i, piece - 1);
-                        load_states<NS>(piece_states(p, ch, at), end[i]);
+                        load_my_states(piece_states(p, ch, at), kLanes * NS, ch.j, end[i]);
                         sum[i] = *piece_sum(p, ch, at);
                     }
 #pragma unroll
@@ -363,13 +416,11 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
                             for (int s = 0; s < NS; ++s) h[s] = __builtin_amdgcn_exp2f(sum[i] * ch.A2[s]) * h[s] + end[i][s];
                 }
             }
-            if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds);
+            if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds, steps);
             if (last) {
                 ch.store_state(p, h);
             } else if (FIRST && ch.live) {
-                float* to = piece_states(p, ch, 0);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) to[s] = h[s];
+                store_my_states(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
             }
         }
         if (!FIRST || piece == 0) zero_frames(p, ch, max(t0, ch.len), te);
@@ -385,7 +436,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
     const long long at = i < last ? i : last;
     const int Dg = p.D / p.G, b = (int)(at / p.D), d = (int)(at % p.D), g = d / Dg;
     Channel<T, NS> ch;
-    ch.init(p, b, g, d - g * Dg);
+    ch.init(p, b, g, d - g * Dg, threadIdx.x & (kLanes - 1));
     ch.live = i <= last;
     float h[NS];
     ch.load_state(p, h);
