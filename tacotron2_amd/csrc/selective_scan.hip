@@ -34,17 +34,16 @@ constexpr int kBlockChannels = 64;  // 4 waves of 16 channels
 
 // A tile of frames in LDS: u, delta, z as they are stored, rows of 64 channels padded so that the four rows that a wave reads
 // at once (lane 16 j + c is on channel c of a frame of its own) lie in different banks; B and C as float32 [frame][4 * NS];
-// the steps dt of 16 frames by channel, each wave's own.
+// beside them, the steps dt by channel, each wave's own.
 template <typename T, int NS>
 struct Tile {
     static constexpr int frames = 64 / (int)sizeof(T), NP = kLanes * NS;
     static constexpr int vec = 16 / (int)sizeof(T), vecs = kBlockChannels / vec;  // vectors of a row
     static constexpr int row = kBlockChannels + 16;                                // elements
+    static constexpr int steps = frames + 4;                                       // floats to a channel, padded
     T rows[3][frames][row];
     float maps[2][frames][NP];
 };
-constexpr int kStepRow = 20;  // floats: 16 frames, padded
-
 template <typename T>
 struct ScanParams {
     Rows<const T> u, delta, z, Bm, Cm;
@@ -216,7 +215,7 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         }
     };
     const int lane = tid & 63, wave = tid >> 6, cl = wave * 16 + (lane & 15);  // the lane's channel of the block's 64
-    float* mine = steps + cl * kStepRow;
+    float* mine = steps + cl * Tl::steps;
     // results leave 16 bytes a lane: 16 channels of a frame on two or four lanes
     constexpr int kOut = 16 / Tl::vec, kOutRows = 64 / kOut;
     const int orow = lane / kOut, ocol = wave * 16 + lane % kOut * Tl::vec;
@@ -228,111 +227,108 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         put(t, tile);
         __syncthreads();
         if (t + Tl::frames < t1) fetch(t + Tl::frames);
-#pragma unroll 1
-        for (int q = 0; q < Tl::frames && t + q < t1; q += 16) {
-            float uv[4], dv[4], xv[4], zv[4], yv[4];
+        // A lane's frames of the tile are j, j + 4, ...: their steps dt, which all four lanes of a channel need, go to LDS.
+        constexpr int L = Tl::frames / 4;
+        float uv[L], xv[L], zv[L], yv[L];
+        {
+            float dv[L];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uv[i] = (float)tile.rows[0][q + 4 * i + ch.j][cl];
-                dv[i] = (float)tile.rows[1][q + 4 * i + ch.j][cl] + bias;
-                if (gate) zv[i] = (float)tile.rows[2][q + 4 * i + ch.j][cl];
+            for (int i = 0; i < L; ++i) {
+                uv[i] = (float)tile.rows[0][4 * i + ch.j][cl];
+                dv[i] = (float)tile.rows[1][4 * i + ch.j][cl] + bias;
+                if (gate) zv[i] = (float)tile.rows[2][4 * i + ch.j][cl];
             }
             if (p.softplus) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dv[i] = softplusf(dv[i]);
+                for (int i = 0; i < L; ++i) dv[i] = softplusf(dv[i]);
             }
-            if (t + q + 16 > t1) {  // frames past the end leave the state as it is: dt = 0
+            if (t + Tl::frames > t1) {  // frames past the end leave the state as it is: dt = 0
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (t + q + 4 * i + ch.j >= t1) uv[i] = dv[i] = 0.f;
+                for (int i = 0; i < L; ++i)
+                    if (t + 4 * i + ch.j >= t1) uv[i] = dv[i] = 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < L; ++i) {
                 xv[i] = dv[i] * uv[i];
                 if (!Y) sum += dv[i];
-            }
-            // A lane has the steps of the frames that it loaded; all four lanes of a channel need each of them
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
                 mine[4 * i + ch.j] = dv[i];
-                if (NS < 4) mine[64 * kStepRow + 4 * i + ch.j] = xv[i];
+                if (NS < 4) mine[kBlockChannels * Tl::steps + 4 * i + ch.j] = xv[i];
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            // F frames at a time: their decays first, exponentials that depend on nothing, then the chain through h; C values
-            // come out of LDS meanwhile.  dt u B of four frames is four outer products, 16 channels by 16 states, on the
-            // matrix unit beside the vector unit's exponentials.
-            constexpr int F = NS >= 16 ? 1 : NS == 8 ? 2 : 4;
-            float cn[2][F][NS], out[4];
-            auto read = [&](int unit, int to) {
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+
+        // F frames at a time, one unit ahead: while the chain through h runs for one unit, the exponentials of the next,
+        // which depend on nothing, fill its gaps, C values come out of LDS, and the matrix unit makes dt u B: of four frames,
+        // four outer products of 16 channels by 16 states.
+        constexpr int F = NS >= 16 ? 1 : NS == 8 ? 2 : 4, units = Tl::frames / F;
+        constexpr int XB = NS >= 16 ? 1 : 2;  // (16 states a lane: no registers for two)
+        float cn[2][F][NS], decay[2][F][NS], out[4];
+        f32x4 xb[XB][4][NS >= 4 ? NS / 4 : 1], dt4[2];
+        auto inputs = [&](int i) {  // of frames 4 i ... 4 i + 3
+            if constexpr (NS >= 4) {
 #pragma unroll
-                for (int f = 0; f < F; ++f)
-                    load_lane_states<NS>(tile.maps[1][q + unit * F + f], ch.j, cn[to][f]);
-            };
-            if (Y) read(0, 0);
-            f32x4 xb[4][NS >= 4 ? NS / 4 : 1];
-            float dt4[4];
+                for (int m = 0; m < NS / 4; ++m) {
+                    typedef float f32x16 __attribute__((ext_vector_type(16)));
+                    const float bn = tile.maps[0][4 * i + ch.j][16 * m + (lane & 15)];
+                    const f32x16 v = __builtin_amdgcn_mfma_f32_16x16x1f32(bn, xv[i], f32x16{}, 0, 0, 0);
 #pragma unroll
-            for (int unit = 0; unit < 16 / F; ++unit) {
-                const int now = unit & 1;
-                if (Y && unit + 1 < 16 / F) read(unit + 1, now ^ 1);
-                if (unit * F % 4 == 0) {
-                    const int i = unit * F / 4;
-                    const f32x4 d4 = *(const f32x4*)&mine[4 * i];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) dt4[k] = d4[k];
-                    if constexpr (NS >= 4) {
-#pragma unroll
-                        for (int m = 0; m < NS / 4; ++m) {
-                            typedef float f32x16 __attribute__((ext_vector_type(16)));
-                            const float bn = tile.maps[0][q + 4 * i + ch.j][16 * m + (lane & 15)];
-                            const f32x16 v = __builtin_amdgcn_mfma_f32_16x16x1f32(bn, xv[i], f32x16{}, 0, 0, 0);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) xb[k][m] = f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
-                        }
-                    } else {
-                        const f32x4 x4 = *(const f32x4*)&mine[64 * kStepRow + 4 * i];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float bn[NS];
-                            load_lane_states<NS>(tile.maps[0][q + 4 * i + k], ch.j, bn);
-#pragma unroll
-                            for (int s = 0; s < NS; ++s) xb[k][0][s] = x4[k] * bn[s];
-                        }
-                    }
+                    for (int k = 0; k < 4; ++k) xb[i % XB][k][m] = f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
                 }
-                float decay[F][NS];
+            } else {
+                const f32x4 x4 = *(const f32x4*)&mine[kBlockChannels * Tl::steps + 4 * i];
 #pragma unroll
-                for (int f = 0; f < F; ++f)
+                for (int k = 0; k < 4; ++k) {
+                    float bn[NS];
+                    load_lane_states<NS>(tile.maps[0][4 * i + k], ch.j, bn);
 #pragma unroll
-                    for (int s = 0; s < NS; ++s) decay[f][s] = __builtin_amdgcn_exp2f(dt4[(unit * F + f) % 4] * ch.A2[s]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    const int k = (unit * F + f) % 4;
-                    float o = 0.f;
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) {
-                        h[s] = __builtin_fmaf(decay[f][s], h[s], xb[k][s / 4][s % 4]);
-                        if (Y) o = s ? __builtin_fmaf(cn[now][f][s], h[s], o) : cn[now][f][s] * h[s];
-                    }
-                    out[k] = o;
+                    for (int s = 0; s < NS; ++s) xb[i % XB][k][0][s] = x4[k] * bn[s];
                 }
-                if (Y && (unit * F + F) % 4 == 0) {
-                    const int i = (unit * F) / 4;
-                    yv[i] = sum_rows(out) + skip * uv[i];
-                }
-                __builtin_amdgcn_sched_barrier(0);
             }
-            if (Y) {
-                if (gate) {
+        };
+        auto prepare = [&](int unit) {
+            if (XB == 2 && unit * F % 4 == 0) inputs(unit * F / 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) yv[i] *= zv[i] * sigmoidf(zv[i]);
-                }
-                // the results take the place of the u that they came from (the same lane's, read above)
+            for (int f = 0; f < F; ++f) {
+                const int k = unit * F + f;
+                if (Y) load_lane_states<NS>(tile.maps[1][k], ch.j, cn[unit & 1][f]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tile.rows[0][q + 4 * i + ch.j][cl] = (T)yv[i];
+                for (int s = 0; s < NS; ++s) decay[unit & 1][f][s] = __builtin_amdgcn_exp2f(dt4[k / 4 % 2][k % 4] * ch.A2[s]);
             }
+        };
+        dt4[0] = *(const f32x4*)&mine[0];
+        if (F == 4) dt4[1] = *(const f32x4*)&mine[4];
+        prepare(0);
+#pragma unroll
+        for (int unit = 0; unit < units; ++unit) {
+            if (unit * F == 16 && t + 16 >= t1) break;
+            const int i = unit * F / 4;
+            __builtin_amdgcn_sched_barrier(0);
+            if (XB == 1 && unit * F % 4 == 0) inputs(i);
+            if (unit + 1 < units) prepare(unit + 1);
+            if ((unit + 2) * F % 4 == 0 && unit + 2 < units) dt4[(unit + 2) * F / 4 % 2] = *(const f32x4*)&mine[(unit + 2) * F];
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                const int k = (unit * F + f) % 4;
+                float o = 0.f;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    h[s] = __builtin_fmaf(decay[unit & 1][f][s], h[s], xb[i % XB][k][s / 4][s % 4]);
+                    if (Y) o = s ? __builtin_fmaf(cn[unit & 1][f][s], h[s], o) : cn[unit & 1][f][s] * h[s];
+                }
+                out[k] = o;
+            }
+            if (Y && (unit * F + F) % 4 == 0) yv[i] = sum_rows(out) + skip * uv[i];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (Y) {
+            if (gate) {
+#pragma unroll
+                for (int i = 0; i < L; ++i) yv[i] *= zv[i] * sigmoidf(zv[i]);
+            }
+            // the results take the place of the u that they came from (the same lane's, read above)
+#pragma unroll
+            for (int i = 0; i < L; ++i) tile.rows[0][4 * i + ch.j][cl] = (T)yv[i];
         }
         if (Y) {
             // a wave reads back what its own lanes wrote: LDS serves a wave's operations in their order
@@ -373,7 +369,7 @@ __device__ __forceinline__ float* piece_sum(const ScanParams<T>& p, const Channe
 template <typename T, int NS, bool FIRST>
 __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
     __shared__ __align__(16) Tile<T, NS> lds[2];
-    __shared__ __align__(16) float steps[(NS < 4 ? 2 : 1) * kBlockChannels * kStepRow];
+    __shared__ __align__(16) float steps[(NS < 4 ? 2 : 1) * kBlockChannels * Tile<T, NS>::steps];
     Channel<T, NS> ch;
     const int g = blockIdx.x / p.blocks_per_group, cb = blockIdx.x % p.blocks_per_group;
     const int piece = FIRST ? blockIdx.y : blockIdx.y + 1;
