@@ -17,7 +17,8 @@ struct CausalParams {
     const int32_t* lengths;
     int B, Tmax, C, w32;
     float slope;
-    int vecs, run, runs;  // vectors of a row, frames a thread walks, threads to a sequence's vector
+    unsigned vecs, runs;
+    int run;  // vectors of a row, threads to a sequence's vector, frames each walks
 };
 
 constexpr int kConvStep = 4;  // frames whose loads are in flight together
@@ -27,10 +28,8 @@ constexpr int kConvStep = 4;  // frames whose loads are in flight together
 template <typename T, int ACT, int K, int V>
 __global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
     typedef typename Unaligned<T, V>::type Vec;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int cv = (int)(id % p.vecs);
-    const long long rest = id / p.vecs;
-    const int r = (int)(rest % p.runs), b = (int)(rest / p.runs);
+    const unsigned id = blockIdx.x * 256 + threadIdx.x, rest = id / p.vecs;
+    const int cv = id % p.vecs, r = p.runs == 1 ? 0 : rest % p.runs, b = p.runs == 1 ? rest : rest / p.runs;
     if (b >= p.B) return;
     const int c = cv * V, n = min(V, p.C - c), len = seq_frames(p.lengths, b, p.Tmax);
     const int t0 = r * p.run, t1 = min(t0 + p.run, p.Tmax);
@@ -185,7 +184,7 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);
         CausalParams<T> p{rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->state_in, (T*)a->state_out,
-                        a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (a->C + V - 1) / V, 0, 0};
+                        a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (unsigned)(a->C + V - 1) / V, 0, 0};
         // long runs read few frames twice (K - 1 a run), short ones give more threads: as long as 2^17 of them allow
         for (p.run = 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;) p.run /= 2;
         p.runs = (a->T + p.run - 1) / p.run;

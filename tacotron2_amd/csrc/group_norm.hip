@@ -8,8 +8,8 @@
 //
 //   frame_norm_kernel     per frame, groups of up to 64 * 8 vectors: L lanes hold a group
 //   group_norm_kernel     a sequence's group(s) in one block's registers: one read, one write, one launch
-//   group_stats_kernel +  a sequence in pieces: count, mean and squared distances of each piece that a block's registers
-//   group_apply_kernel    hold; then the pieces are put together and x is read a second time
+//   group_stats_kernel +  a sequence in pieces: count, mean and squared distances of each, batch by batch; then the pieces are
+//   group_apply_kernel    put together and x is read a second time
 //   wide_norm_kernel      what none of them holds: groups of more channels than a block holds at once
 //
 // A vector is the largest power of two of channels, 16 bytes at most, that divides a group: it never holds two groups.
@@ -18,7 +18,7 @@
 namespace mv {
 
 int check_sequence(const char* who, int B, int T, int C, int dtype) {
-    if (B < 0 || T < 0 || C < 1) {
+    if (B < 0 || T < 0 || T > 1 << 30 || C < 1 || C > 1 << 30) {
         set_error("%s: bad sizes (B=%d, T=%d, channels=%d)", who, B, T, C);
         return MV_EINVAL;
     }
@@ -138,8 +138,8 @@ struct Place {
     int row, rows, c, mine, gv;
     bool in;  // false: a thread without a row, or past the last vector of a row; it loads what its neighbour does
 
-    __device__ __forceinline__ Place(const NormParams<T>& p) {
-        const int tile0 = blockIdx.x * p.tile, v = threadIdx.x % p.tile;
+    __device__ __forceinline__ Place(const NormParams<T>& p, int tile) {
+        const int tile0 = tile * p.tile, v = threadIdx.x % p.tile;
         gv = p.C / p.G / V;
         rows = blockDim.x / p.tile;
         row = min((int)threadIdx.x / p.tile, rows - 1);
@@ -195,55 +195,95 @@ struct Held {
 
 constexpr int kNormThreads = 1024;
 
-// Grid (tiles, sequences): whole groups of a whole sequence.
+// One block to a tile of a sequence: whole groups of it, all frames.  Blocks go to the 8 XCDs in turn; here each XCD gets a
+// run of tiles, so that tiles that share a 128-byte line meet in one L2.
 template <typename T, int V, int NI, int ACT>
 __global__ __launch_bounds__(kNormThreads) void group_norm_kernel(NormParams<T> p) {
     __shared__ float red[2 * kNormThreads];
     typedef typename Unaligned<T, V>::type Vec;
-    const Place<T, V> at(p);
+    const unsigned work = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int b = work / p.tiles;
+    if (b >= p.B) return;
+    const Place<T, V> at(p, work - b * p.tiles);
     Held<T, V, NI> h;
-    for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
-        const int len = seq_frames(p.lengths, b, p.Tmax);
-        const float count = (float)len * (float)(p.C / p.G);
-        if (len) h.take(p, at, b, 0, len, count, red);
-        const float rstd = 1.f / sqrtf(h.m2 / count + p.eps);
-        float w[V], bias[V];
-        load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
-        load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
+    const int len = seq_frames(p.lengths, b, p.Tmax);
+    const float count = (float)len * (float)(p.C / p.G);
+    if (len) h.take(p, at, b, 0, len, count, red);
+    const float rstd = 1.f / sqrtf(h.m2 / count + p.eps);
+    float w[V], bias[V];
+    load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
+    load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int t = at.row + i * at.rows;
-            Vec y;
-            if (t < len) {
-                y = normalise<T, V, ACT>(h.x[i], h.mean, rstd, w, bias, p.slope);
-            } else {
+    for (int i = 0; i < NI; ++i) {
+        const int t = at.row + i * at.rows;
+        Vec y;
+        if (t < len) {
+            y = normalise<T, V, ACT>(h.x[i], h.mean, rstd, w, bias, p.slope);
+        } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = (T)0.f;
-            }
-            if (at.in && t < p.Tmax) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, 0, i, p.Tmax) = y;
-            __builtin_amdgcn_sched_barrier(0);  // one vector after the other: the registers hold the tile, not 16 results
+            for (int e = 0; e < V; ++e) y[e] = (T)0.f;
         }
+        if (at.in && t < p.Tmax) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, 0, i, p.Tmax) = y;
+        __builtin_amdgcn_sched_barrier(0);  // one vector after the other: the registers hold the tile, not 16 results
     }
 }
 
-// Grid (tiles, pieces, sequences): statistics of a piece of a sequence.
-template <typename T, int V, int NI>
+// Grid (tiles, pieces, sequences): statistics of a piece of a sequence.  A thread takes kStatRows vectors at a time: their
+// mean, their squared distances from it, and both into what it has so far (n, mean, m2 of the values seen:
+// mean' = mean + d n2 / n', m2' = m2 + q + d^2 n n2 / n' with d the distance of the means); the block's threads are put
+// together the same way at the end.
+constexpr int kStatRows = 8;
+template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void group_stats_kernel(NormParams<T> p) {
     __shared__ float red[2 * kNormThreads];
-    const Place<T, V> at(p);
-    Held<T, V, NI> h;
+    typedef typename Unaligned<T, V>::type Vec;
+    const Place<T, V> at(p, blockIdx.x);
+    const int Cg = p.C / p.G;
     for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
         const int len = seq_frames(p.lengths, b, p.Tmax);
         const int t0 = blockIdx.y * p.piece, t1 = min(t0 + p.piece, len);
-        const int Cg = p.C / p.G;
+        float n = 0.f, mean = 0.f, m2 = 0.f;
+        for (int t = t0; t < t1; t += kStatRows * at.rows) {
+            Vec x[kStatRows];
+#pragma unroll
+            for (int i = 0; i < kStatRows; ++i) x[i] = *(const Vec*)at.at(p.x.row(b, 0), p.x.rs, t, i, t1);
+            // this thread's frames of the batch: t + row, t + row + rows, ...
+            const int mine = at.in ? min(kStatRows, max(0, (t1 - t - at.row + at.rows - 1) / at.rows)) : 0;
+            const float n2 = (float)(mine * V);
+            if (mine > 0) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < kStatRows; ++i)
+                    if (i < mine)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) s += (float)x[i][e];
+                const float mu = s / n2;
+                float q = 0.f;
+#pragma unroll
+                for (int i = 0; i < kStatRows; ++i)
+                    if (i < mine)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const float d = (float)x[i][e] - mu;
+                            q += d * d;
+                        }
+                const float all = n + n2, d = mu - mean, part = n2 / all;
+                mean += d * part;
+                m2 += q + d * d * n * part;
+                n = all;
+            }
+        }
         const float count = t1 > t0 ? (float)(t1 - t0) * (float)Cg : 0.f;
-        h.mean = h.m2 = 0.f;
-        if (t1 > t0) h.take(p, at, b, t0, t1, count, red);
+        if (t1 > t0) {
+            const float mu = group_total(n * mean, red, at.rows, p.tile, at.gv, at.mine) / count, d = mean - mu;
+            m2 = group_total(n > 0.f ? m2 + n * d * d : 0.f, red, at.rows, p.tile, at.gv, at.mine);
+            mean = mu;
+        }
         if (at.in && at.row == 0 && at.c % Cg == 0) {
             const long long i = ((long long)b * p.G + at.c / Cg) * p.pieces + blockIdx.y;
             p.n[i] = count;
-            p.mean[i] = h.mean;
-            p.m2[i] = h.m2;
+            p.mean[i] = mean;
+            p.m2[i] = m2;
         }
     }
 }
@@ -274,7 +314,7 @@ template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T> p) {
     __shared__ float stat[2 * kNormThreads];
     typedef typename Unaligned<T, V>::type Vec;
-    const Place<T, V> at(p);
+    const Place<T, V> at(p, blockIdx.x);
     float w[V], bias[V];
     load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
     load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
@@ -317,11 +357,11 @@ __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T>
 // Each frame's groups by themselves: L lanes to a group, NI vectors to a lane.  A slot of L lanes keeps its group (and its
 // weights) and walks the frames.
 template <typename T, int V, int NI, int ACT>
-__global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L, long long slots) {
+__global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L, unsigned slots) {
     typedef typename Unaligned<T, V>::type Vec;
-    const long long slot = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const unsigned slot = (blockIdx.x * 256 + threadIdx.x) >> (31 - __builtin_clz(L));
     if (slot >= slots) return;  // (whole slots leave: L divides 64)
-    const int l = threadIdx.x & (L - 1), Cg = p.C / p.G, nv = Cg / V, g = (int)(slot % p.G);
+    const int l = threadIdx.x & (L - 1), Cg = p.C / p.G, nv = Cg / V, g = slot % p.G;
     float w[NI][V], bias[NI][V];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -329,9 +369,9 @@ __global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L,
         load_weights<T, V>(p.w, p.w32, c, 1.f, w[i]);
         load_weights<T, V>(p.b, p.w32, c, 0.f, bias[i]);
     }
-    const long long frames = (long long)p.B * p.Tmax;
-    for (long long f = slot / p.G; f < frames; f += slots / p.G) {
-        const int b = (int)(f / p.Tmax), t = (int)(f - (long long)b * p.Tmax);
+    const unsigned frames = p.B * p.Tmax;
+    for (unsigned f = slot / p.G; f < frames; f += slots / p.G) {
+        const int b = f / p.Tmax, t = f - b * p.Tmax;
         T* to = p.y.row(b, t) + g * Cg;
         if (t >= seq_frames(p.lengths, b, p.Tmax)) {
 #pragma unroll
@@ -460,32 +500,37 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     if (gv > kNormThreads) return s;
     const long long far = std::max(a->x.row_stride, a->y.row_stride);
     auto fits = [&](long long frames) { return (frames * far + a->C) * size < 1ll << 31; };  // Place's offsets
-    // whole groups side by side until a row of the tile is a 128-byte line
+    // Whole groups side by side.  A tile of a whole sequence: rows of 32 bytes at least, as many blocks as that gives (two
+    // and more to a CU, one loading while another reduces or stores), 128 bytes where there are blocks in plenty.
+    const int most = std::min(row, kNormThreads);
+    auto grow = [&](int bytes) {
+        while (s.tile * s.V * size < bytes && s.tile + gv <= most) s.tile += gv;
+        s.tiles = ceil_div(row, s.tile);
+    };
     s.tile = gv;
-    while (s.tile * s.V * size < 128 && s.tile + gv <= std::min(row, kNormThreads)) s.tile += gv;
-    for (int threads = 256; threads <= kNormThreads; threads *= 2) {
-        if (threads < s.tile) continue;
-        const int n = ceil_div(a->T, threads / s.tile);
-        if (n <= (threads < kNormThreads ? 4 : 16) && fits(threads / s.tile * 16)) {
+    grow(32);
+    if ((long long)s.tiles * a->B > 4096) grow(128);
+    for (s.threads = 64; s.threads <= kNormThreads; s.threads *= 2) {
+        if (s.threads < s.tile) continue;
+        const int n = ceil_div(a->T, s.threads / s.tile);
+        if (n <= (s.threads < kNormThreads ? 8 : 16) && fits(s.threads / s.tile * 16ll) &&
+            (long long)s.tiles * a->B * s.threads < 1ll << 31) {
             s.kind = NORM_HELD;
-            s.threads = threads;
-            s.NI = n <= 1 ? 1 : n <= 4 ? 4 : 16;
-            s.tiles = ceil_div(row, s.tile);
+            s.NI = n <= 1 ? 1 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
             return s;
         }
     }
-    // pieces: blocks of 1024 threads, as large as leaves two for each CU
-    s.threads = kNormThreads;
-    s.tiles = ceil_div(row, s.tile);
+    // Pieces: full lines, and enough of them for four blocks to a CU.
+    grow(128);
+    s.threads = std::max(256, pow2_at_least(s.tile, kNormThreads));
     const int rows = s.threads / s.tile;
-    for (s.NI = 16;; s.NI = 4) {
-        s.piece = rows * s.NI;
-        s.pieces = ceil_div(a->T, s.piece);
-        if (s.NI == 4 || (long long)s.tiles * s.pieces * a->B >= 512) break;
-    }
-    s.apply_piece = rows * 8;
-    if (ceil_div(a->T, s.apply_piece) > 65535 || !fits(rows * s.NI)) return s;
+    const long long want = std::max(1ll, 1024 / ((long long)s.tiles * a->B));
+    s.piece = rows * kStatRows * std::max(1, ceil_div(a->T, want * rows * kStatRows));
+    s.pieces = ceil_div(a->T, s.piece);
+    s.apply_piece = rows * 16;
+    if (s.pieces > 65535 || ceil_div(a->T, s.apply_piece) > 65535 || !fits(rows * 16ll)) return s;
     s.kind = NORM_PIECES;
+    s.NI = 1;
     s.bytes = ((size_t)a->B * a->groups * s.pieces * 3 * 4 + 255) / 256 * 256;
     return s;
 }
@@ -532,17 +577,23 @@ static int launch_norm(const mv_group_norm_args* a, const NormPlan& s, NormParam
             if constexpr (NI <= 8) {
                 const long long frames = (long long)a->B * a->T, most = 2048ll * 256 / s.L / a->groups;
                 const long long slots = std::min(frames, std::max(1ll, most)) * a->groups;
+                if (frames >= 1ll << 31 || slots * s.L >= 1ll << 31) {
+                    set_error("mv_group_norm: more than 2^31 frames, or groups of a frame, in one call");
+                    return MV_EINVAL;
+                }
                 hipLaunchKernelGGL((frame_norm_kernel<T, V, NI, ACT>), dim3((unsigned)((slots * s.L + 255) / 256)), dim3(256), 0,
-                                   stream, p, s.L, slots);
+                                   stream, p, s.L, (unsigned)slots);
             }
-        } else if constexpr (NI == 1 || NI == 4 || NI == 16) {
+        } else if constexpr (NI != 2) {
             p.tile = s.tile;
+            p.tiles = s.tiles;
             if (s.kind == NORM_HELD) {
-                hipLaunchKernelGGL((group_norm_kernel<T, V, NI, ACT>), dim3(s.tiles, B16), dim3(s.threads), 0, stream, p);
-            } else if constexpr (NI > 1) {
+                hipLaunchKernelGGL((group_norm_kernel<T, V, NI, ACT>), dim3((s.tiles * a->B + 7) / 8 * 8), dim3(s.threads), 0,
+                                   stream, p);
+            } else if constexpr (NI == 1) {
                 p.piece = s.piece;
                 p.pieces = s.pieces;
-                hipLaunchKernelGGL((group_stats_kernel<T, V, NI>), dim3(s.tiles, s.pieces, B16), dim3(s.threads), 0, stream, p);
+                hipLaunchKernelGGL((group_stats_kernel<T, V>), dim3(s.tiles, s.pieces, B16), dim3(s.threads), 0, stream, p);
                 MV_HIP(hipGetLastError());
                 p.piece = s.apply_piece;
                 hipLaunchKernelGGL((group_apply_kernel<T, V, ACT>), dim3(s.tiles, ceil_div(a->T, s.apply_piece), B16),

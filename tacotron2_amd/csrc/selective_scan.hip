@@ -443,42 +443,45 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
     }
 }
 
-// A few frames of many sequences (decode steps): no LDS, no barrier; what counts is the state, read and written once.
+// A few frames of many sequences (decode steps): no LDS, no barrier; what counts is the state, read and written once.  Here
+// the four lanes of a channel stand side by side, so that a wave's states are one piece of memory.  Grid (64 channels,
+// sequences).
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 2;
-    const long long last = (long long)p.B * p.D - 1;
-    const long long at = i < last ? i : last;
-    const int Dg = p.D / p.G, b = (int)(at / p.D), d = (int)(at % p.D), g = d / Dg;
-    Channel<T, NS> ch;
-    ch.init(p, b, g, d - g * Dg, threadIdx.x & (kLanes - 1));
-    ch.live = i <= last;
-    float h[NS];
-    ch.load_state(p, h);
-    const float bias = p.bias ? p.bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
-    for (int t = 0; t < p.Tmax; ++t) {
-        float v = 0.f;
-        if (t < ch.len) {
-            const float u = (float)p.u.row(b, t)[d];
-            float dt = (float)p.delta.row(b, t)[d] + bias;
-            float bn[NS], cn[NS];
-            load_my_states(p.Bm.row(b, t) + g * p.Bg, p.N, ch.j, bn);
-            load_my_states(p.Cm.row(b, t) + g * p.Cg, p.N, ch.j, cn);
-            const float z = p.z.p ? (float)p.z.row(b, t)[d] : 0.f;
-            if (p.softplus) dt = softplusf(dt);
-            const float x = dt * u;
+    const int c = blockIdx.x * kBlockChannels + (threadIdx.x >> 2), d = min(c, p.D - 1), Dg = p.D / p.G;
+    const int g = p.G == 1 ? 0 : d / Dg;
+    if (__builtin_amdgcn_readfirstlane(c) >= p.D) return;
+    for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+        Channel<T, NS> ch;
+        ch.init(p, b, g, d - g * Dg, threadIdx.x & (kLanes - 1));
+        ch.live = c < p.D;
+        float h[NS];
+        ch.load_state(p, h);
+        const float bias = p.bias ? p.bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
+        for (int t = 0; t < p.Tmax; ++t) {
+            float v = 0.f;
+            if (t < ch.len) {
+                const float u = (float)p.u.row(b, t)[d];
+                float dt = (float)p.delta.row(b, t)[d] + bias;
+                float bn[NS], cn[NS];
+                load_my_states(p.Bm.row(b, t) + g * p.Bg, p.N, ch.j, bn);
+                load_my_states(p.Cm.row(b, t) + g * p.Cg, p.N, ch.j, cn);
+                const float z = p.z.p ? (float)p.z.row(b, t)[d] : 0.f;
+                if (p.softplus) dt = softplusf(dt);
+                const float x = dt * u;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                h[s] = __builtin_amdgcn_exp2f(dt * ch.A2[s]) * h[s] + x * bn[s];
-                v += cn[s] * h[s];
+                for (int s = 0; s < NS; ++s) {
+                    h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * ch.A2[s]), h[s], x * bn[s]);
+                    v += cn[s] * h[s];
+                }
+                v += quad<0xB1>(v), v += quad<0x4E>(v);
+                v += skip * u;
+                if (p.z.p) v *= z * sigmoidf(z);
             }
-            v += quad<0xB1>(v), v += quad<0x4E>(v);  // (the four lanes of a channel are in this branch together)
-            v += skip * u;
-            if (p.z.p) v *= z * sigmoidf(z);
+            if (ch.live && ch.j == 0) p.y.row(b, t)[d] = (T)v;
         }
-        if (ch.live && ch.j == 0) p.y.row(b, t)[d] = (T)v;
+        ch.store_state(p, h);
     }
-    ch.store_state(p, h);
 }
 
 // Calls of up to this many frames take the step kernel.
@@ -516,8 +519,8 @@ static ScanPlan scan_plan(const mv_selective_scan_args* a) {
 template <typename T, int NS>
 static int launch_scan(ScanParams<T> p, hipStream_t stream) {
     if (p.Tmax <= kStepFrames) {
-        const long long blocks = ((long long)p.B * p.D * kLanes + 255) / 256;
-        hipLaunchKernelGGL((scan_step_kernel<T, NS>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        const dim3 grid((p.D + kBlockChannels - 1) / kBlockChannels, (unsigned)std::min(p.B, 65535));
+        hipLaunchKernelGGL((scan_step_kernel<T, NS>), grid, dim3(256), 0, stream, p);
         MV_HIP(hipGetLastError());
         return MV_OK;
     }

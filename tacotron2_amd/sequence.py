@@ -40,21 +40,28 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, slo
                   ahead and is the same in a whole call as frame by frame
     activation    None, "silu", "relu", "leaky_relu" (with `slope`) or "tanh"
     """
-    x, shape, B, T, ch, sb, st = _data("group_norm", "x", x)
+    x, shape, B, T, ch, sb, st, dtype, dev = _data("group_norm", "x", x)
     if groups < 1 or ch % groups:
         raise RuntimeError(f"group_norm: {ch} channels do not split into {groups} groups")
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps < _INF:
         raise RuntimeError("group_norm: eps must be finite and not negative")
     act, slope = _activation("group_norm", activation, slope)
-    weight, bias, wtype = _weights("group_norm", x, weight, (ch,), bias, ch)
-    if torch.is_grad_enabled():
+    wtype, wp, bp = 0, 0, 0
+    if weight is not None or bias is not None:
+        weight, bias = _one_type(weight, bias)
+        if weight is not None:
+            weight, wtype, wp = _weight("group_norm", "weight", weight, (ch,), dtype, dev)
+        if bias is not None:
+            bias, wtype, bp = _weight("group_norm", "bias", bias, (ch,), dtype, dev)
+    if _grad():
         _no_grad("group_norm", x, weight, bias)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = _like(x) if x.is_contiguous() else _empty(shape, dtype=dtype, device=x.device)
     if B and T:
-        lengths = _lengths(lengths, B, T, x)
-        _call(_native.GROUP_NORM, x, T > 1, _native.GROUP_NORM.pack(
-            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, _ptr(weight), _ptr(bias), _ptr(lengths), B, T, ch, groups,
-            _DTYPES[x.dtype], wtype, 1 if per_frame else 0, act, slope, eps))
+        if lengths is not None:
+            lengths = _lengths(lengths, B, T, x)
+        _call(_native.GROUP_NORM, x, dev, T > 1, _native.GROUP_NORM.pack(
+            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, wp, bp, 0 if lengths is None else lengths.data_ptr(), B, T, ch,
+            groups, _DTYPES[dtype], wtype, 1 if per_frame else 0, act, slope, eps))
     return y
 
 
@@ -66,22 +73,32 @@ def causal_conv(x, weight, bias=None, activation=None, slope=0.1, state=None, st
     weight     [C, K] or [C, 1, K] (a depthwise `torch.nn.Conv1d`'s), 1 <= K <= 8, float32 or x's type; bias [C] or None
     state      [B, K - 1, C] of x's type, the frames before the first, oldest first (None: zeros); state_out likewise
     """
-    x, shape, B, T, ch, sb, st = _data("causal_conv", "x", x)
+    x, shape, B, T, ch, sb, st, dtype, dev = _data("causal_conv", "x", x)
     w = weight.shape
     K = w[-1] if len(w) > 1 else 0
     if not (w == (ch, K) or w == (ch, 1, K)) or not 1 <= K <= MAX_TAPS:
         raise RuntimeError(f"causal_conv: expected a weight [{ch}, K] with 1 <= K <= {MAX_TAPS}, got {tuple(w)}")
     act, slope = _activation("causal_conv", activation, slope)
-    weight, bias, wtype = _weights("causal_conv", x, weight, w, bias, ch)
-    _states("causal_conv", x, state, state_out, (B, K - 1, ch), x.dtype)
-    if torch.is_grad_enabled():
+    weight, bias = _one_type(weight, bias)
+    weight, wtype, wp = _weight("causal_conv", "weight", weight, w, dtype, dev)
+    bp = sp = op = 0
+    if bias is not None:
+        bias, wtype, bp = _weight("causal_conv", "bias", bias, (ch,), dtype, dev)
+    if state is not None:
+        sp = _state("causal_conv", "state", state, (B, K - 1, ch), dtype, dev)
+    if state_out is state:
+        op = sp
+    elif state_out is not None:
+        op = _state("causal_conv", "state_out", state_out, (B, K - 1, ch), dtype, dev)
+    if _grad():
         _no_grad("causal_conv", x, weight, bias, state, state_out)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = _like(x) if x.is_contiguous() else _empty(shape, dtype=dtype, device=x.device)
     if B and (T or state_out is not None):
-        lengths = _lengths(lengths, B, T, x)
-        _call(_native.CAUSAL_CONV, x, False, _native.CAUSAL_CONV.pack(
-            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(state_out),
-            _ptr(lengths), B, T, ch, K, _DTYPES[x.dtype], wtype, act, slope))
+        if lengths is not None:
+            lengths = _lengths(lengths, B, T, x)
+        _call(_native.CAUSAL_CONV, x, dev, False, _native.CAUSAL_CONV.pack(
+            x.data_ptr(), sb, st, y.data_ptr(), T * ch, ch, wp, bp, sp, op, 0 if lengths is None else lengths.data_ptr(), B, T,
+            ch, K, _DTYPES[dtype], wtype, act, slope))
     return y
 
 
@@ -99,111 +116,127 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     state         [B, D, N] float32 (None: zeros); state_out likewise
     u, delta, z, B, C share one type.
     """
-    u, shape, nb, T, ch, sb, st = _data("selective_scan", "u", u)
-    for name, t in (("delta", delta), ("z", z)):
-        if t is not None and t.shape != shape:
-            raise RuntimeError(f"selective_scan: {name} has shape {tuple(t.shape)}, u {tuple(shape)}")
-    a = A.shape
-    if len(a) != 2 or a[0] != ch or not 1 <= a[1] <= MAX_STATES:
+    u, shape, nb, T, ch, sb, st, dtype, dev = _data("selective_scan", "u", u)
+    a, m = A.shape, B.shape
+    N = a[-1]
+    if not 1 <= N <= MAX_STATES or a != (ch, N):
         raise RuntimeError(f"selective_scan: expected A [{ch}, N] with 1 <= N <= {MAX_STATES}, got {tuple(a)}")
-    N = a[1]
-    lead, m = shape[:-1], B.shape
     G = m[-2] if len(m) == len(shape) + 1 else 1
-    if C.shape != m or not (m == (*lead, N) or m == (*lead, G, N)):
-        raise RuntimeError(f"selective_scan: B and C must be {list(lead)} + [{N}] or [G, {N}], got {tuple(m)} and "
+    if C.shape != m or m[-1] != N or m[:len(shape) - 1] != shape[:-1] or len(m) not in (len(shape), len(shape) + 1):
+        raise RuntimeError(f"selective_scan: B and C must be {list(shape[:-1])} + [{N}] or [G, {N}], got {tuple(m)} and "
                            f"{tuple(C.shape)}")
     if G < 1 or ch % G:
         raise RuntimeError(f"selective_scan: {ch} channels do not split into {G} groups")
-    dev = u.get_device()
-    for name, t in (("delta", delta), ("z", z), ("B", B), ("C", C)):
-        if t is not None and (t.dtype != u.dtype or t.get_device() != dev):
-            raise RuntimeError(f"selective_scan: {name} must be {u.dtype} on {u.device} like u, got {t.dtype} on {t.device}")
-    A = _float32("selective_scan", u, "A", A, (ch, N))
-    D = _float32("selective_scan", u, "D", D, (ch,))
-    delta_bias = _float32("selective_scan", u, "delta_bias", delta_bias, (ch,))
-    _states("selective_scan", u, state, state_out, (nb, ch, N), torch.float32)
-    if torch.is_grad_enabled():
+    delta, sd = _rows("delta", delta, shape, dtype, dev)
+    B, sB = _rows("B", B, m, dtype, dev)
+    C, sC = _rows("C", C, m, dtype, dev)
+    zp, sz = 0, _NO_STRIDES
+    if z is not None:
+        z, sz = _rows("z", z, shape, dtype, dev)
+        zp = z.data_ptr()
+    Dp = bp = sp = op = 0
+    A = _float32("A", A, a, dev)
+    if D is not None:
+        D = _float32("D", D, (ch,), dev)
+        Dp = D.data_ptr()
+    if delta_bias is not None:
+        delta_bias = _float32("delta_bias", delta_bias, (ch,), dev)
+        bp = delta_bias.data_ptr()
+    if state is not None:
+        sp = _state("selective_scan", "state", state, (nb, ch, N), torch.float32, dev)
+    if state_out is state:
+        op = sp
+    elif state_out is not None:
+        op = _state("selective_scan", "state_out", state_out, (nb, ch, N), torch.float32, dev)
+    if _grad():
         _no_grad("selective_scan", u, delta, z, B, C, A, D, delta_bias, state, state_out)
-    y = torch.empty(shape, dtype=u.dtype, device=u.device)
+    y = _like(u) if u.is_contiguous() else _empty(shape, dtype=dtype, device=u.device)
     if nb and (T or state_out is not None):
-        lengths = _lengths(lengths, nb, T, u)
-        delta, sd = _adjacent(delta)
-        z, sz = _adjacent(z) if z is not None else (None, (0, 0, 0))
-        B, sB = _adjacent(B)
-        C, sC = _adjacent(C)
-        f = len(shape) == 3  # with a frame axis
-        _call(_native.SELECTIVE_SCAN, u, T > 1, _native.SELECTIVE_SCAN.pack(
-            u.data_ptr(), sb, st, delta.data_ptr(), sd[0], sd[1] if f else 0, _ptr(z), sz[0], sz[1] if f else 0,
-            B.data_ptr(), sB[0], sB[1] if f else 0, C.data_ptr(), sC[0], sC[1] if f else 0, sB[-2] if G > 1 else 0,
-            sC[-2] if G > 1 else 0, y.data_ptr(), T * ch, ch, A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(state),
-            _ptr(state_out), _ptr(lengths), nb, T, ch, N, G, _DTYPES[u.dtype], 1 if delta_softplus else 0))
+        if lengths is not None:
+            lengths = _lengths(lengths, nb, T, u)
+        t = 1 if len(shape) == 3 else 0  # where a row's stride stands; a frame without the axis is one row, whatever the stride
+        gB, gC = (sB[-2], sC[-2]) if G > 1 else (0, 0)
+        _call(_native.SELECTIVE_SCAN, u, dev, T > 1, _native.SELECTIVE_SCAN.pack(
+            u.data_ptr(), sb, st, delta.data_ptr(), sd[0], t and sd[t], zp, sz[0], t and sz[t], B.data_ptr(), sB[0], t and sB[t],
+            C.data_ptr(), sC[0], t and sC[t], gB, gC, y.data_ptr(), T * ch, ch, A.data_ptr(), Dp, bp, sp, op,
+            0 if lengths is None else lengths.data_ptr(), nb, T, ch, N, G, _DTYPES[dtype], 1 if delta_softplus else 0))
     return y
 
 
-# --- arguments (checks are plain comparisons: a decode step's call is short against what Python adds to it) -----------
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _adjacent(t):
-    """-> (t with channels side by side, its strides)"""
-    s = t.stride()
-    if s[-1] == 1 or t.shape[-1] == 1:
-        return t, s
-    t = t.contiguous()
-    return t, t.stride()
+# --- arguments.  A decode step's call is short against what Python adds to it: checks are plain comparisons, messages are made
+# --- where one fails.
+_INF, _NO_STRIDES = float("inf"), (0, 0, 0)
+_empty, _like, _grad = torch.empty, torch.empty_like, torch.is_grad_enabled
 
 
 def _data(who, name, x):
-    """-> (x with adjacent channels, its shape, B, T, channels, batch and row stride)"""
-    shape = x.shape
+    """-> (x with adjacent channels, its shape, B, T, channels, batch stride, row stride, type, device index)"""
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    if dev < 0:
+        raise RuntimeError(f"tacotron2_amd.sequence.{who} computes on an MI355X only (no CPU fallback)")
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"{who}: {name} must be float32, bfloat16 or float16, got {dtype}")
+    s = x.stride()
     if len(shape) not in (2, 3) or shape[-1] < 1:
         raise RuntimeError(f"{who}: {name} must be [B, T, channels] or [B, channels], got {tuple(shape)}")
-    if not x.is_cuda:
-        raise RuntimeError(f"tacotron2_amd.sequence.{who} computes on an MI355X only (no CPU fallback)")
-    if x.dtype not in _DTYPES:
-        raise RuntimeError(f"{who}: {name} must be float32, bfloat16 or float16, got {x.dtype}")
-    x, s = _adjacent(x)
+    if s[-1] != 1 and shape[-1] != 1:
+        x = x.contiguous()
+        s = x.stride()
     if len(shape) == 3:
-        return x, shape, shape[0], shape[1], shape[2], s[0], s[1]
-    return x, shape, shape[0], 1, shape[1], s[0], 0
+        return x, shape, shape[0], shape[1], shape[2], s[0], s[1], dtype, dev
+    return x, shape, shape[0], 1, shape[1], s[0], 0, dtype, dev
+
+
+def _rows(name, t, shape, dtype, dev):
+    """-> (t with adjacent channels, its strides)"""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise RuntimeError(f"selective_scan: {name} must be {list(shape)}, {dtype}, on the device of u; got {list(t.shape)}, "
+                           f"{t.dtype}, on {t.device}")
+    s = t.stride()
+    if s[-1] != 1 and shape[-1] != 1:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s
 
 
 def _activation(who, activation, slope):
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"{who}: unknown activation {activation!r} (one of {sorted(a for a in _ACTIVATIONS if a)}, None)")
-    return _ACTIVATIONS[activation], 0.0 if activation == "relu" else float(slope)
+    return act, 0.0 if activation == "relu" else slope
 
 
-def _weights(who, x, weight, shape, bias, ch):
-    """-> (weight, bias, MV_DTYPE_* of both): contiguous, of one type, float32 or x's."""
+def _one_type(weight, bias):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        weight, bias = weight.float(), bias.float()
-    wtype = 0
-    for name, t, want in (("weight", weight, shape), ("bias", bias, (ch,))):
-        if t is not None:
-            if t.shape != want or t.get_device() != x.get_device() or not (t.dtype == torch.float32 or t.dtype == x.dtype):
-                raise RuntimeError(f"{who}: {name} must be {list(want)}, float32 or {x.dtype}, on {x.device}; got "
-                                   f"{list(t.shape)}, {t.dtype}, on {t.device}")
-            wtype = _DTYPES[t.dtype]
-    return (weight if weight is None else weight.contiguous()), (bias if bias is None else bias.contiguous()), wtype
+        return weight.float(), bias.float()
+    return weight, bias
 
 
-def _float32(who, x, name, t, shape):
-    if t is None:
-        return None
-    if t.shape != shape or t.get_device() != x.get_device() or t.dtype not in _DTYPES:
-        raise RuntimeError(f"{who}: {name} must be {list(shape)} floats on {x.device}, got {list(t.shape)}, {t.dtype}, on "
-                           f"{t.device}")
-    return t.contiguous() if t.dtype == torch.float32 else t.float().contiguous()
+def _weight(who, name, t, shape, dtype, dev):
+    """-> (t contiguous, its MV_DTYPE_*, its address)"""
+    if t.shape != shape or t.get_device() != dev or not (t.dtype == torch.float32 or t.dtype == dtype):
+        raise RuntimeError(f"{who}: {name} must be {list(shape)}, float32 or {dtype}, on the device of x; got {list(t.shape)}, "
+                           f"{t.dtype}, on {t.device}")
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t, _DTYPES[t.dtype], t.data_ptr()
 
 
-def _states(who, x, state, state_out, shape, dtype):
-    for name, t in (("state", state), ("state_out", state_out)):
-        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != x.get_device()
-                              or not t.is_contiguous()):
-            raise RuntimeError(f"{who}: {name} must be contiguous {list(shape)}, {dtype}, on {x.device}; got "
-                               f"{list(t.shape)}, {t.dtype}, on {t.device}")
+def _float32(name, t, shape, dev):
+    if t.shape != shape or t.get_device() != dev or t.dtype not in _DTYPES:
+        raise RuntimeError(f"selective_scan: {name} must be {list(shape)} floats on the device of u, got {list(t.shape)}, "
+                           f"{t.dtype}, on {t.device}")
+    if t.dtype != torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _state(who, name, t, shape, dtype, dev):
+    """-> its address"""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+        raise RuntimeError(f"{who}: {name} must be contiguous {list(shape)}, {dtype}, on the device of the data; got "
+                           f"{list(t.shape)}, {t.dtype}, on {t.device}")
+    return t.data_ptr()
 
 
 def _no_grad(who, *tensors):
@@ -213,8 +246,6 @@ def _no_grad(who, *tensors):
 
 
 def _lengths(lengths, B, T, x):
-    if lengths is None:
-        return None
     if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
         if lengths.numel() != B or lengths.is_floating_point():
             raise RuntimeError("lengths must hold B frame counts in [0, T]")
@@ -225,14 +256,13 @@ def _lengths(lengths, B, T, x):
     return _native.device_lengths(lengths, B, T, x.device)
 
 
-def _call(op, x, scratch, args):
+def _call(op, x, dev, scratch, args):
     """One call of the library on x's device and its current stream.  Scratch (which calls of one frame do without) comes from
     torch's allocator, in a capture from the graph's own pool: a new piece for every call, so that no two calls or graphs
     share one."""
-    dev = x.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            return _call(op, x, scratch, args)
+            return _call(op, x, dev, scratch, args)
     if op.fn is None:
         op.bind()
     stream = torch._C._cuda_getCurrentRawStream(dev)
@@ -240,7 +270,7 @@ def _call(op, x, scratch, args):
         rc = op.fn(args, stream)
     else:
         n = op.fn_workspace(args) if scratch else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        rc = op.fn(args, _ptr(ws), n, stream)
+        ws = _empty(n, dtype=torch.uint8, device=x.device) if n else None
+        rc = op.fn(args, 0 if ws is None else ws.data_ptr(), n, stream)
     if rc:
         _native.check(rc, op.name)
