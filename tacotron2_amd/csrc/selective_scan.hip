@@ -490,9 +490,9 @@ constexpr int kStepFrames = 4;
 // Pieces that the frames of each sequence are cut into.
 static int scan_pieces(int B, int T, int D, int G) {
     const long long waves = (long long)B * G * ((D / G + 15) / 16);
-    if (waves >= 1024 || T < 128) return 1;
+    if (waves >= 1024 || T < 96) return 1;
     long long n = 2048 / waves;
-    n = std::min<long long>(n, T / 64);
+    n = std::min<long long>(n, T / 32);
     n = std::min<long long>(n, 128);
     return n < 3 ? 1 : (int)n;
 }
