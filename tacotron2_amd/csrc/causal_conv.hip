@@ -18,16 +18,19 @@ struct CausalParams {
     int B, Tmax, C, w32;
     float slope;
     unsigned vecs, runs;
-    int run;  // vectors of a row, threads to a sequence's vector, frames each walks
+    int run, past;  // vectors of a row, threads to a sequence's vector, frames each walks; results past the L2
 };
 
-constexpr int kConvStep = 4;  // frames whose loads are in flight together
+// frames whose loads are in flight together (more taps leave registers for fewer)
+template <int K>
+constexpr int kConvStep = K <= 4 ? 8 : 4;
 
 // A thread walks `run` frames of V adjacent channels with the K - 1 frames before in registers.  The thread of a sequence's
 // first run also moves the state on: it alone reads state_in, before it writes state_out.
 template <typename T, int ACT, int K, int V>
 __global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
     typedef typename Unaligned<T, V>::type Vec;
+    constexpr int kStep = kConvStep<K>;
     const unsigned id = blockIdx.x * 256 + threadIdx.x, rest = id / p.vecs;
     const int cv = id % p.vecs, r = p.runs == 1 ? 0 : rest % p.runs, b = p.runs == 1 ? rest : rest / p.runs;
     if (b >= p.B) return;
@@ -96,20 +99,20 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) bias[e] = p.bias && e < n ? load_weight<T>(p.bias, p.w32, c + e) : 0.f;
     }
-    float x[K - 1 + kConvStep][V];
+    float x[K - 1 + kStep][V];
 #pragma unroll
     for (int k = 0; k + 1 < K; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) x[k][e] = (float)carry[k][e];
     const int live = min(t1, len);
     int t = t0;
-    for (; t < live; t += kConvStep) {
-        Vec raw[kConvStep];
+    for (; t < live; t += kStep) {
+        Vec raw[kStep];
 #pragma unroll
-        for (int u = 0; u < kConvStep; ++u)
+        for (int u = 0; u < kStep; ++u)
             if (t + u < live) raw[u] = load_some<T, V>(from + (t + u) * p.x.rs, n);
 #pragma unroll
-        for (int u = 0; u < kConvStep; ++u) {
+        for (int u = 0; u < kStep; ++u) {
             if (t + u >= live) break;
             Vec y;
 #pragma unroll
@@ -120,17 +123,17 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
                 for (int k = 0; k < K; ++k) v += w[e * K + k] * x[u + k][e];
                 y[e] = (T)activate<ACT>(v, p.slope);
             }
-            store_some<T, V>(to + (t + u) * p.y.rs, y, n);
+            store_some<T, V>(to + (t + u) * p.y.rs, y, n, p.past);
         }
 #pragma unroll
         for (int k = 0; k + 1 < K; ++k)
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[k][e] = x[k + kConvStep][e];
+            for (int e = 0; e < V; ++e) x[k][e] = x[k + kStep][e];
     }
     Vec zero;
 #pragma unroll
     for (int e = 0; e < V; ++e) zero[e] = (T)0.f;
-    for (t = max(t0, len); t < t1; ++t) store_some<T, V>(to + t * p.y.rs, zero, n);
+    for (t = max(t0, len); t < t1; ++t) store_some<T, V>(to + t * p.y.rs, zero, n, p.past);
 }
 
 template <typename F>
@@ -184,7 +187,7 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);
         CausalParams<T> p{rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->state_in, (T*)a->state_out,
-                        a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (unsigned)(a->C + V - 1) / V, 0, 0};
+                        a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (unsigned)(a->C + V - 1) / V, 0, 0, pass_by_l2(a->y, a->B, a->T, a->C, a->dtype)};
         // long runs read few frames twice (K - 1 a run), short ones give more threads: as long as 2^17 of them allow
         for (p.run = 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;) p.run /= 2;
         p.runs = (a->T + p.run - 1) / p.run;

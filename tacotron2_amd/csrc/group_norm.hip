@@ -64,7 +64,7 @@ struct NormParams {
     const void *w, *b;
     const int32_t* lengths;
     float *n, *mean, *m2;  // pieces' statistics [B][G][pieces]
-    int B, Tmax, C, G, w32;
+    int B, Tmax, C, G, w32, past;  // past: results past the L2
     float slope, eps;
     int tile, tiles;     // vectors of a row to a block, blocks to a row
     int piece, pieces;   // frames to a block, blocks to a sequence
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kNormThreads) void group_norm_kernel(NormParams<T> 
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] = (T)0.f;
         }
-        if (at.in && t < p.Tmax) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, 0, i, p.Tmax) = y;
+        if (at.in && t < p.Tmax) store_vec<T, V>(at.at(p.y.row(b, 0), p.y.rs, 0, i, p.Tmax), y, p.past);
         __builtin_amdgcn_sched_barrier(0);  // one vector after the other: the registers hold the tile, not 16 results
     }
 }
@@ -308,8 +308,7 @@ __device__ __forceinline__ void join_pieces(const float* n, const float* mean, c
     if (lane == 0) *out_mean = mu, *out_rstd = 1.f / sqrtf(q / N + eps);
 }
 
-// Grid (tiles, pieces, sequences), the last ones first: what the statistics read last is still in the caches.  `piece` is
-// this launch's own, a multiple of 4 * rows frames.
+// Grid (tiles, pieces, sequences).  `piece` is this launch's own, a multiple of 4 * rows frames.
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T> p) {
     __shared__ float stat[2 * kNormThreads];
@@ -319,10 +318,9 @@ __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T>
     load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
     load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
     const int Cg = p.C / p.G, g0 = blockIdx.x * p.tile * V / Cg, groups = p.tile * V / Cg;
-    const int piece = gridDim.y - 1 - blockIdx.y;
-    for (int bb = blockIdx.z; bb < p.B; bb += gridDim.z) {
-        const int b = p.B - 1 - bb, len = seq_frames(p.lengths, b, p.Tmax);
-        const int t0 = piece * p.piece, te = min(t0 + p.piece, p.Tmax), live = min(te, len);
+    for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
+        const int len = seq_frames(p.lengths, b, p.Tmax);
+        const int t0 = blockIdx.y * p.piece, te = min(t0 + p.piece, p.Tmax), live = min(te, len);
         __syncthreads();
         if (t0 < live)
             for (int g = threadIdx.x >> 6; g < groups; g += blockDim.x >> 6)
@@ -348,7 +346,7 @@ __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T>
 #pragma unroll
                     for (int e = 0; e < V; ++e) y[e] = (T)0.f;
                 }
-                if (at.in && f < te) *(Vec*)at.at(p.y.row(b, 0), p.y.rs, t, i, te) = y;
+                if (at.in && f < te) store_vec<T, V>(at.at(p.y.row(b, 0), p.y.rs, t, i, te), y, p.past);
             }
         }
     }
@@ -473,6 +471,7 @@ __global__ __launch_bounds__(256) void wide_norm_kernel(NormParams<T> p, int per
 enum { NORM_FRAME, NORM_HELD, NORM_PIECES, NORM_WIDE };
 struct NormPlan {
     int kind, V, NI, threads, tile, tiles, piece, pieces, apply_piece, L;
+    bool past;
     size_t bytes;
 };
 
@@ -508,7 +507,9 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
         s.tiles = ceil_div(row, s.tile);
     };
     s.tile = gv;
-    grow(32);
+    s.past = pass_by_l2(a->y, a->B, a->T, a->C, a->dtype);
+    grow(s.past ? 64 : 32);
+    s.past = s.past && (s.tile * s.V * size) % 64 == 0;
     if ((long long)s.tiles * a->B > 4096) grow(128);
     for (s.threads = 64; s.threads <= kNormThreads; s.threads *= 2) {
         if (s.threads < s.tile) continue;
@@ -520,14 +521,14 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
             return s;
         }
     }
-    // Pieces: full lines, and enough of them for four blocks to a CU.
+    // Pieces: full lines, and enough of them for eight blocks to a CU (padded ones leave at once).
     grow(128);
     s.threads = std::max(256, pow2_at_least(s.tile, kNormThreads));
     const int rows = s.threads / s.tile;
-    const long long want = std::max(1ll, 1024 / ((long long)s.tiles * a->B));
+    const long long want = std::max(1ll, 2048 / ((long long)s.tiles * a->B));
     s.piece = rows * kStatRows * std::max(1, ceil_div(a->T, want * rows * kStatRows));
     s.pieces = ceil_div(a->T, s.piece);
-    s.apply_piece = rows * 16;
+    s.apply_piece = rows * 32;
     if (s.pieces > 65535 || ceil_div(a->T, s.apply_piece) > 65535 || !fits(rows * 16ll)) return s;
     s.kind = NORM_PIECES;
     s.NI = 1;
@@ -665,6 +666,7 @@ int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace
         p.C = a->C;
         p.G = a->groups;
         p.w32 = a->weight_dtype == MV_DTYPE_F32;
+        p.past = plan.past;
         p.eps = a->eps;
         return by_activation(a->activation, a->slope, &p.slope, [&](auto act) {
             return launch_norm<T, decltype(act)::value>(a, plan, p, (hipStream_t)stream);
