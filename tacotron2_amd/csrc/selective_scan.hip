@@ -59,6 +59,10 @@ template <int CTRL>
 __device__ __forceinline__ float quad(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
+// lane k's value in all four (k is a constant once the loop around it is unrolled)
+__device__ __forceinline__ float quad_lane(float v, int k) {
+    return k == 0 ? quad<0x00>(v) : k == 1 ? quad<0x55>(v) : k == 2 ? quad<0xAA>(v) : quad<0xFF>(v);
+}
 
 // Lane j's NS of the N values at p, as floats; zeros where it has fewer.
 template <typename T, int NS>
@@ -94,6 +98,24 @@ __device__ __forceinline__ void store_my_states(float* p, int N, int j, const fl
     }
 }
 
+// A of channel d for exponentials to base 2.  Clamped to finite: 0 * inf must not make a NaN of a frame past the end, whose dt
+// is 0.
+template <typename T, int NS>
+__device__ __forceinline__ void load_decays(const ScanParams<T>& p, int d, int j, float (&A2)[NS]) {
+    load_my_states(p.A + (long long)d * p.N, p.N, j, A2);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) A2[s] = fminf(fmaxf(A2[s] * kLog2e, -3e38f), 3e38f);
+}
+template <int NS>
+__device__ __forceinline__ void load_state(const float* from, int N, int j, float (&h)[NS]) {
+    if (from) {
+        load_my_states(from, N, j, h);
+    } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) h[s] = 0.f;
+    }
+}
+
 // The calling thread's channel and states.
 template <typename T, int NS>
 struct Channel {
@@ -107,24 +129,7 @@ struct Channel {
         live = c < Dg;
         d = g * Dg + min(c, Dg - 1);
         len = seq_frames(p.lengths, b, p.Tmax);
-        load_my_states(p.A + (long long)d * p.N, p.N, j, A2);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            // clamped to finite: 0 * inf must not make a NaN of a frame past the end, whose dt is 0
-            const float a = A2[s] * kLog2e;
-            A2[s] = a < -3e38f ? -3e38f : (a > 3e38f ? 3e38f : a);
-        }
-    }
-    __device__ __forceinline__ void load_state(const ScanParams<T>& p, float (&h)[NS]) const {
-        if (p.state_in) {
-            load_my_states(p.state_in + ((long long)b * p.D + d) * p.N, p.N, j, h);
-        } else {
-#pragma unroll
-            for (int s = 0; s < NS; ++s) h[s] = 0.f;
-        }
-    }
-    __device__ __forceinline__ void store_state(const ScanParams<T>& p, const float (&h)[NS]) const {
-        if (p.state_out && live) store_my_states(p.state_out + ((long long)b * p.D + d) * p.N, p.N, j, h);
+        load_decays(p, d, j, A2);
     }
 };
 
@@ -412,7 +417,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             }
         } else if (FIRST || t0 < ch.len) {
             if (FIRST) {
-                ch.load_state(p, h);
+                load_state(p.state_in ? p.state_in + ((long long)b * p.D + ch.d) * p.N : nullptr, p.N, ch.j, h);
             } else {
                 load_my_states(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
                 constexpr int kBatch = NS >= 16 ? 2 : 8;  // pieces whose loads are in flight together
@@ -433,7 +438,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             }
             if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds, steps);
             if (last) {
-                ch.store_state(p, h);
+                if (p.state_out && ch.live) store_my_states(p.state_out + ((long long)b * p.D + ch.d) * p.N, p.N, ch.j, h);
             } else if (FIRST && ch.live) {
                 store_my_states(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
             }
@@ -443,46 +448,88 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
     }
 }
 
+// a[k] of four values, each spread over a quad's four lanes: lane k gets the sum of a[k]
+__device__ __forceinline__ float sum_quad(const float (&a)[4], int j) {
+    const bool o1 = j & 1, o2 = j & 2;
+    const float x = (o1 ? a[1] : a[0]) + quad<0xB1>(o1 ? a[0] : a[1]);
+    const float y = (o1 ? a[3] : a[2]) + quad<0xB1>(o1 ? a[2] : a[3]);
+    return (o2 ? y : x) + quad<0x4E>(o2 ? x : y);
+}
+
 // A few frames of many sequences (decode steps): no LDS, no barrier; what counts is the state, read and written once.  Here
-// the four lanes of a channel stand side by side, so that a wave's states are one piece of memory.  Grid (64 channels,
-// sequences).
+// the four lanes of a channel stand side by side, so that a wave's states are one piece of memory, and a quad of lanes has Q
+// channels: with Q = 4, lane j brings u, delta and z of the quad's channel j, makes its step and hands it around, and B and C
+// are loaded once for the four (a wave's memory instructions, not its bytes, are what a call of 16 states waits for: 14
+// instead of 32 for 64 channels).  With 8 and more states a lane, one channel fills the registers.  Grid
+// (channels, sequences): a block keeps its channels' A and walks sequences.
+template <int NS>
+constexpr int kQuadChannels = NS <= 4 ? 4 : 1;
+
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
-    const int c = blockIdx.x * kBlockChannels + (threadIdx.x >> 2), d = min(c, p.D - 1), Dg = p.D / p.G;
-    const int g = p.G == 1 ? 0 : d / Dg;
-    if (__builtin_amdgcn_readfirstlane(c) >= p.D) return;
+    constexpr int Q = kQuadChannels<NS>;
+    const int j = threadIdx.x & (kLanes - 1), c0 = (blockIdx.x * 64 + (threadIdx.x >> 2)) * Q, Dg = p.D / p.G;
+    if (__builtin_amdgcn_readfirstlane(c0) >= p.D) return;
+    const int mine = Q == 4 ? c0 + j : c0, d = min(mine, p.D - 1);  // the channel whose u, delta, z and y are this lane's
+    const bool live = mine < p.D, together = p.G == 1 || (Q == 4 && Dg % 4 == 0);
+    int dk[Q], gk[Q];
+    float A2[Q][NS];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        dk[k] = min(c0 + k, p.D - 1);
+        gk[k] = p.G == 1 ? 0 : dk[k] / Dg;
+        load_decays(p, dk[k], j, A2[k]);
+    }
+    const float bias = p.bias ? p.bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
     for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
-        Channel<T, NS> ch;
-        ch.init(p, b, g, d - g * Dg, threadIdx.x & (kLanes - 1));
-        ch.live = c < p.D;
-        float h[NS];
-        ch.load_state(p, h);
-        const float bias = p.bias ? p.bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
+        const int len = seq_frames(p.lengths, b, p.Tmax);
+        const long long state = (long long)b * p.D * p.N;
+        float h[Q][NS];
+#pragma unroll
+        for (int k = 0; k < Q; ++k) load_state(p.state_in ? p.state_in + state + dk[k] * p.N : nullptr, p.N, j, h[k]);
         for (int t = 0; t < p.Tmax; ++t) {
             float v = 0.f;
-            if (t < ch.len) {
-                const float u = (float)p.u.row(b, t)[d];
-                float dt = (float)p.delta.row(b, t)[d] + bias;
-                float bn[NS], cn[NS];
-                load_my_states(p.Bm.row(b, t) + g * p.Bg, p.N, ch.j, bn);
-                load_my_states(p.Cm.row(b, t) + g * p.Cg, p.N, ch.j, cn);
+            if (t < len) {
+                const float u = (float)p.u.row(b, t)[d], raw = (float)p.delta.row(b, t)[d] + bias;
                 const float z = p.z.p ? (float)p.z.row(b, t)[d] : 0.f;
-                if (p.softplus) dt = softplusf(dt);
-                const float x = dt * u;
+                float bn[NS], cn[NS], out[Q];
+                auto maps = [&](int k) {
+                    load_my_states(p.Bm.row(b, t) + gk[k] * p.Bg, p.N, j, bn);
+                    load_my_states(p.Cm.row(b, t) + gk[k] * p.Cg, p.N, j, cn);
+                };
+                maps(0);
+                const float dt = p.softplus ? softplusf(raw) : raw, x = dt * u;
 #pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * ch.A2[s]), h[s], x * bn[s]);
-                    v += cn[s] * h[s];
+                for (int k = 0; k < Q; ++k) {
+                    const float dtk = Q == 4 ? quad_lane(dt, k) : dt, xk = Q == 4 ? quad_lane(x, k) : x;
+                    if (k && !together) maps(k);
+                    out[k] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        h[k][s] = __builtin_fmaf(__builtin_amdgcn_exp2f(dtk * A2[k][s]), h[k][s], xk * bn[s]);
+                        out[k] += cn[s] * h[k][s];
+                    }
                 }
-                v += quad<0xB1>(v), v += quad<0x4E>(v);
+                if constexpr (Q == 4) {
+                    v = sum_quad(out, j);
+                } else {
+                    v = out[0] + quad<0xB1>(out[0]);
+                    v += quad<0x4E>(v);
+                }
                 v += skip * u;
                 if (p.z.p) v *= z * sigmoidf(z);
             }
-            if (ch.live && ch.j == 0) p.y.row(b, t)[d] = (T)v;
+            if (live && (Q == 4 || j == 0)) p.y.row(b, t)[d] = (T)v;
         }
-        ch.store_state(p, h);
+        if (p.state_out) {
+#pragma unroll
+            for (int k = 0; k < Q; ++k)
+                if (c0 + k < p.D) store_my_states(p.state_out + state + dk[k] * p.N, p.N, j, h[k]);
+        }
     }
 }
+
+constexpr int kStepBlocks = 2048;  // of the step kernel: eight to a CU, each then walks B * D / 64 / 2048 sequences
 
 // Calls of up to this many frames take the step kernel.
 constexpr int kStepFrames = 4;
@@ -519,7 +566,8 @@ static ScanPlan scan_plan(const mv_selective_scan_args* a) {
 template <typename T, int NS>
 static int launch_scan(ScanParams<T> p, hipStream_t stream) {
     if (p.Tmax <= kStepFrames) {
-        const dim3 grid((p.D + kBlockChannels - 1) / kBlockChannels, (unsigned)std::min(p.B, 65535));
+        const int x = (p.D + 64 * kQuadChannels<NS> - 1) / (64 * kQuadChannels<NS>);
+        const dim3 grid(x, (unsigned)std::min(p.B, std::max(1, std::min(65535, kStepBlocks / x))));
         hipLaunchKernelGGL((scan_step_kernel<T, NS>), grid, dim3(256), 0, stream, p);
         MV_HIP(hipGetLastError());
         return MV_OK;

@@ -121,8 +121,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     N = a[-1]
     if not 1 <= N <= MAX_STATES or a != (ch, N):
         raise RuntimeError(f"selective_scan: expected A [{ch}, N] with 1 <= N <= {MAX_STATES}, got {tuple(a)}")
-    G = m[-2] if len(m) == len(shape) + 1 else 1
-    if C.shape != m or m[-1] != N or m[:len(shape) - 1] != shape[:-1] or len(m) not in (len(shape), len(shape) + 1):
+    axes = len(shape)
+    G = m[-2] if len(m) == axes + 1 else 1
+    if C.shape != m or len(m) - axes not in (0, 1) or m[-1] != N or m[0] != nb or (axes == 3 and m[1] != T):
         raise RuntimeError(f"selective_scan: B and C must be {list(shape[:-1])} + [{N}] or [G, {N}], got {tuple(m)} and "
                            f"{tuple(C.shape)}")
     if G < 1 or ch % G:
@@ -154,11 +155,12 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     if nb and (T or state_out is not None):
         if lengths is not None:
             lengths = _lengths(lengths, nb, T, u)
-        t = 1 if len(shape) == 3 else 0  # where a row's stride stands; a frame without the axis is one row, whatever the stride
+        # a row's stride is the second one; without the frame axis there is one row, wherever the next would be
+        td, tz, tB, tC = (sd[1], sz[1], sB[1], sC[1]) if axes == 3 else (0, 0, 0, 0)
         gB, gC = (sB[-2], sC[-2]) if G > 1 else (0, 0)
         _call(_native.SELECTIVE_SCAN, u, dev, T > 1, _native.SELECTIVE_SCAN.pack(
-            u.data_ptr(), sb, st, delta.data_ptr(), sd[0], t and sd[t], zp, sz[0], t and sz[t], B.data_ptr(), sB[0], t and sB[t],
-            C.data_ptr(), sC[0], t and sC[t], gB, gC, y.data_ptr(), T * ch, ch, A.data_ptr(), Dp, bp, sp, op,
+            u.data_ptr(), sb, st, delta.data_ptr(), sd[0], td, zp, sz[0], tz, B.data_ptr(), sB[0], tB, C.data_ptr(), sC[0], tC,
+            gB, gC, y.data_ptr(), T * ch, ch, A.data_ptr(), Dp, bp, sp, op,
             0 if lengths is None else lengths.data_ptr(), nb, T, ch, N, G, _DTYPES[dtype], 1 if delta_softplus else 0))
     return y
 
