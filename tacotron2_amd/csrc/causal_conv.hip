@@ -161,8 +161,8 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         return MV_EINVAL;
     }
     if (int rc = check_sequence(who, a->B, a->T, a->C, a->dtype)) return rc;
-    if (a->K < 1 || a->K > 8) {
-        set_error("%s: %d taps (1 to 8)", who, a->K);
+    if (a->K < 1 || a->K > 8 || a->C > 1 << 27) {
+        set_error("%s: %d taps (1 to 8), or more than 2^27 channels", who, a->K);
         return MV_EINVAL;
     }
     if (!a->weight || (a->weight_dtype != MV_DTYPE_F32 && a->weight_dtype != a->dtype)) {
@@ -173,6 +173,10 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         set_error("%s: unknown activation %d", who, a->activation);
         return MV_EINVAL;
     }
+    const size_t size = dtype_size(a->dtype), wsize = dtype_size(a->weight_dtype);
+    for (auto [p, bytes] : {std::pair<const void*, size_t>{a->weight, wsize}, {a->bias, wsize}, {a->state_in, size},
+                            {a->state_out, size}, {a->lengths, 4}})
+        if (int rc = check_aligned(who, p, bytes)) return rc;
     const long long states = (long long)a->B * (a->K - 1) * a->C;
     if (int rc = check_states(who, a->state_in, a->state_out, states * (long long)dtype_size(a->dtype))) return rc;
     if (a->B == 0) return MV_OK;
@@ -181,7 +185,7 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
             using T = decltype(t);
             return carry_state((const T*)a->state_in, (T*)a->state_out, states, (hipStream_t)stream);
         });
-    if (int rc = check_rows(who, "x", a->x, a->dtype)) return rc;
+    if (int rc = check_rows(who, "x", a->x, a->T, a->dtype)) return rc;
     if (int rc = check_output_rows(who, a->y, a->B, a->T, a->C, a->dtype)) return rc;
     return by_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
@@ -192,7 +196,7 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         for (p.run = 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;) p.run /= 2;
         p.runs = (a->T + p.run - 1) / p.run;
         const long long blocks = ((long long)a->B * p.runs * p.vecs + 255) / 256;
-        if (blocks > 0xffffff) {
+        if (blocks > 0x7fffff) {
             set_error("%s: too many frames for one call", who);
             return MV_EINVAL;
         }

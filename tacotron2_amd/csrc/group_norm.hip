@@ -29,8 +29,15 @@ int check_sequence(const char* who, int B, int T, int C, int dtype) {
     return MV_OK;
 }
 
-int check_rows(const char* who, const char* what, const mv_rows& r, int dtype) {
-    if (!r.ptr || ((uintptr_t)r.ptr % dtype_size(dtype)) != 0 || r.batch_stride < 0 || r.row_stride < 0 || r.row_stride > 1 << 25) {
+int check_aligned(const char* who, const void* p, size_t bytes) {
+    if ((uintptr_t)p % bytes == 0) return MV_OK;
+    set_error("%s: a pointer is not aligned to its elements", who);
+    return MV_EINVAL;
+}
+
+int check_rows(const char* who, const char* what, const mv_rows& r, int T, int dtype) {
+    if (!r.ptr || ((uintptr_t)r.ptr % dtype_size(dtype)) != 0 || r.batch_stride < 0 || r.row_stride < 0 ||
+        (T > 1 && r.row_stride > 1 << 25)) {
         set_error("%s: %s needs an aligned pointer, strides >= 0 and a row stride of at most 2^25", who, what);
         return MV_EINVAL;
     }
@@ -48,7 +55,7 @@ int check_states(const char* who, const void* in, const void* out, long long byt
 }
 
 int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, int dtype) {
-    if (int rc = check_rows(who, "the output", r, dtype)) return rc;
+    if (int rc = check_rows(who, "the output", r, T, dtype)) return rc;
     if (!rows_disjoint(r, B, T, C)) {
         set_error("%s: the output's rows overlap (batch_stride %lld, row_stride %lld)", who, (long long)r.batch_stride,
                   (long long)r.row_stride);
@@ -642,8 +649,12 @@ size_t mv_group_norm_workspace(const mv_group_norm_args* a) {
 int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = check_group_norm(a)) return rc;
     if (a->B == 0 || a->T == 0) return MV_OK;
-    if (int rc = check_rows("mv_group_norm", "x", a->x, a->dtype)) return rc;
+    if (int rc = check_rows("mv_group_norm", "x", a->x, a->T, a->dtype)) return rc;
     if (int rc = check_output_rows("mv_group_norm", a->y, a->B, a->T, a->C, a->dtype)) return rc;
+    const size_t wsize = dtype_size(a->weight_dtype);
+    if (int rc = check_aligned("mv_group_norm", a->weight, wsize)) return rc;
+    if (int rc = check_aligned("mv_group_norm", a->bias, wsize)) return rc;
+    if (int rc = check_aligned("mv_group_norm", a->lengths, 4)) return rc;
     const NormPlan plan = norm_plan(a);
     if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 255) != 0)) {
         set_error("mv_group_norm: workspace: need %zu bytes, 256-byte aligned (got %zu)", plan.bytes, workspace_bytes);

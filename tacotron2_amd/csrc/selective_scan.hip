@@ -12,7 +12,7 @@ __device__ __forceinline__ float softplusf(float x) {
     constexpr float kLn2 = 0.693147180559945309f;
     const float a = fabsf(x), t = a * -kLog2e, lost = __builtin_fmaf(a, -kLog2e, -t);
     float e = __builtin_amdgcn_exp2f(t);
-    e = __builtin_fmaf(e, lost * kLn2, e);
+    e = e > 0.f ? __builtin_fmaf(e, lost * kLn2, e) : e;  // (what an infinity lost is no number)
     const float w = 1.f + e;
     return fmaxf(x, 0.f) + __builtin_fmaf(__builtin_amdgcn_logf(w), kLn2, e - (w - 1.f));
 }
@@ -41,6 +41,7 @@ struct Tile {
     T rows[3][frames][row];
     float maps[2][frames][NP];
 };
+
 template <typename T>
 struct ScanParams {
     Rows<const T> u, delta, z, Bm, Cm;
@@ -104,7 +105,10 @@ template <typename T, int NS>
 __device__ __forceinline__ void load_decays(const ScanParams<T>& p, int d, int j, float (&A2)[NS]) {
     load_my_states(p.A + (long long)d * p.N, p.N, j, A2);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) A2[s] = fminf(fmaxf(A2[s] * kLog2e, -3e38f), 3e38f);
+    for (int s = 0; s < NS; ++s) {
+        const float a = A2[s] * kLog2e;
+        A2[s] = a < -3e38f ? -3e38f : (a > 3e38f ? 3e38f : a);  // (a NaN stays one)
+    }
 }
 template <int NS>
 __device__ __forceinline__ void load_state(const float* from, int N, int j, float (&h)[NS]) {
@@ -116,7 +120,7 @@ __device__ __forceinline__ void load_state(const float* from, int N, int j, floa
     }
 }
 
-// The calling thread's channel and states.
+// The calling thread's channel.
 template <typename T, int NS>
 struct Channel {
     int b, g, d, j, len;
@@ -218,6 +222,7 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         }
     };
     const int lane = tid & 63, wave = tid >> 6, cl = wave * 16 + (lane & 15);  // the lane's channel of the block's 64
+    const bool idle = __builtin_amdgcn_readfirstlane(c0 + wave * 16) >= p.D / p.G;  // a wave past the group's last channel only loads
     float* mine = steps + cl * Tl::steps;
     // results leave 16 bytes a lane: 16 channels of a frame on two or four lanes
     constexpr int kOut = 16 / Tl::vec, kOutRows = 64 / kOut;
@@ -230,6 +235,7 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         put(t, tile);
         __syncthreads();
         if (t + Tl::frames < t1) fetch(t + Tl::frames);
+        if (idle) continue;
         // A lane's frames of the tile are j, j + 4, ...: their steps dt, which all four lanes of a channel need, go to LDS.
         constexpr int L = Tl::frames / 4;
         float uv[L], xv[L], zv[L], yv[L];
@@ -348,7 +354,7 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
     return sum;
 }
 
-// zeros for the frames past a sequence's end, by the whole block
+// zeros for the frames past a sequence's end
 template <typename T, int NS>
 __device__ __forceinline__ void zero_frames(const ScanParams<T>& p, const Channel<T, NS>& ch, int t0, int t1) {
     T* yb = p.y.row(ch.b, 0) + ch.d;
@@ -433,7 +439,8 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
                     for (int i = 0; i < kBatch; ++i)
                         if (k + i < piece)
 #pragma unroll
-                            for (int s = 0; s < NS; ++s) h[s] = __builtin_amdgcn_exp2f(sum[i] * ch.A2[s]) * h[s] + end[i][s];
+                            for (int s = 0; s < NS; ++s)  // (a state of zero stays zero whatever its factor overflows to)
+                                h[s] = (h[s] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sum[i] * ch.A2[s]) * h[s]) + end[i][s];
                 }
             }
             if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds, steps);
@@ -622,13 +629,20 @@ int mv_selective_scan(const mv_selective_scan_args* a, void* workspace, size_t w
         set_error("%s: needs A", who);
         return MV_EINVAL;
     }
+    for (const void* f : {(const void*)a->A, (const void*)a->Dskip, (const void*)a->delta_bias, (const void*)a->state_in,
+                          (const void*)a->state_out, (const void*)a->lengths})
+        if (int rc = check_aligned(who, f, 4)) return rc;
+    if (a->Bg_stride < 0 || a->Cg_stride < 0) {
+        set_error("%s: group strides must be >= 0", who);
+        return MV_EINVAL;
+    }
     const struct {
         const char* name;
         const mv_rows* r;
     } ins[] = {{"u", &a->u}, {"delta", &a->delta}, {"z", &a->z}, {"Bm", &a->Bm}, {"Cm", &a->Cm}};
     for (const auto& in : ins)
         if (in.r != &a->z || in.r->ptr)
-            if (int rc = check_rows(who, in.name, *in.r, a->dtype)) return rc;
+            if (int rc = check_rows(who, in.name, *in.r, a->T, a->dtype)) return rc;
     if (int rc = check_output_rows(who, a->y, a->B, a->T, a->D, a->dtype)) return rc;
     const ScanPlan plan = scan_plan(a);
     if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 255) != 0)) {

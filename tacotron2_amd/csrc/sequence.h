@@ -151,7 +151,8 @@ inline int carry_state(const T* in, T* out, long long n, hipStream_t stream) {
 
 // host-side checks shared by the operators; `who` is the entry point's name
 int check_sequence(const char* who, int B, int T, int C, int dtype);
-int check_rows(const char* who, const char* what, const mv_rows& r, int dtype);
+int check_aligned(const char* who, const void* p, size_t bytes);
+int check_rows(const char* who, const char* what, const mv_rows& r, int T, int dtype);
 int check_states(const char* who, const void* in, const void* out, long long bytes);
 int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, int dtype);
 

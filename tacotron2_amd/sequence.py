@@ -10,14 +10,17 @@ projection's output, `[T, B, C]` memory: taken as they lie; a tensor whose chann
 tensor without the frame axis, `[B, channels]`, is one frame of each sequence: a decode step.  Arithmetic is float32 and is
 rounded once, at the result.
 
-`lengths=` (host or device, as in the vocoders) holds the true frame counts of a right-padded batch: row b equals the call
-on `x[b, :lengths[b]]`, whatever the padding holds, and its frames past the end are written as 0.  Host-side lengths outside
-`[0, T]` raise, lengths already on the device are clamped there.
+`lengths=` (host or device, as in the vocoders) holds the true frame counts of a right-padded batch: row b is the call on
+`x[b, :lengths[b]]` (to float32 rounding: how sums are cut goes by the size of the call), whatever the padding holds, and its
+frames past the end are written as 0.  Host-side lengths outside `[0, T]` raise, lengths already on the device are clamped
+there.
 
 `state=` is where a sequence stands before the call (None: at its beginning), `state_out=` a tensor that receives where it
 stands after its last true frame; they may be the same tensor, so a sequence cut into calls (prompt, then frame by frame)
-gives the results of one call.  With `state_out` given and no allocation of the caller's in between, a call can be captured
-into a HIP graph.  These are synthesis-time layers: inputs that require a gradient are refused (outside `no_grad`).
+gives the results of one call: the convolution bit for bit, the scan to float32 rounding.  Calls can be captured into HIP
+graphs; a decode step on static tensors with its state replaced in place is one kernel.
+
+These are synthesis-time layers: inputs that require a gradient are refused (outside `no_grad`).
 """
 from __future__ import annotations
 
@@ -118,8 +121,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     """
     u, shape, nb, T, ch, sb, st, dtype, dev = _data("selective_scan", "u", u)
     a, m = A.shape, B.shape
-    N = a[-1]
-    if not 1 <= N <= MAX_STATES or a != (ch, N):
+    N = a[1] if len(a) == 2 else 0
+    if not 1 <= N <= MAX_STATES or a[0] != ch:
         raise RuntimeError(f"selective_scan: expected A [{ch}, N] with 1 <= N <= {MAX_STATES}, got {tuple(a)}")
     axes = len(shape)
     G = m[-2] if len(m) == axes + 1 else 1
@@ -155,8 +158,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     if nb and (T or state_out is not None):
         if lengths is not None:
             lengths = _lengths(lengths, nb, T, u)
-        # a row's stride is the second one; without the frame axis there is one row, wherever the next would be
-        td, tz, tB, tC = (sd[1], sz[1], sB[1], sC[1]) if axes == 3 else (0, 0, 0, 0)
+        # a row's stride is the second one; of a single row it says nothing
+        td, tz, tB, tC = (sd[1], sz[1], sB[1], sC[1]) if T > 1 else (0, 0, 0, 0)
         gB, gC = (sB[-2], sC[-2]) if G > 1 else (0, 0)
         _call(_native.SELECTIVE_SCAN, u, dev, T > 1, _native.SELECTIVE_SCAN.pack(
             u.data_ptr(), sb, st, delta.data_ptr(), sd[0], td, zp, sz[0], tz, B.data_ptr(), sB[0], tB, C.data_ptr(), sC[0], tC,
@@ -185,7 +188,8 @@ def _data(who, name, x):
         x = x.contiguous()
         s = x.stride()
     if len(shape) == 3:
-        return x, shape, shape[0], shape[1], shape[2], s[0], s[1], dtype, dev
+        T = shape[1]
+        return x, shape, shape[0], T, shape[2], s[0], s[1] if T > 1 else 0, dtype, dev  # (of one row the stride says nothing)
     return x, shape, shape[0], 1, shape[1], s[0], 0, dtype, dev
 
 

@@ -337,6 +337,11 @@ SCAN = [
     (1, 500, 24, 4, 24, F16, True, True, None),  # a group to each channel
     (2, 257, 640, 16, 4, BF16, True, True, [257, 256]),
     (40, 70, 512, 16, 1, BF16, True, False, None),
+    (1, 6000, 16, 16, 1, F32, True, True, None),  # as many pieces as there are
+    (2, 200, 48, 16, 16, BF16, True, True, [200, 77]),  # groups of three channels
+    (3, 2, 30, 20, 2, F16, True, True, [2, 1, 0]),  # few frames, more states than a quad of channels holds
+    (2, 3, 20, 16, 5, F32, True, True, None),  # few frames, quads of channels in two groups
+    (300, 40, 16, 8, 1, BF16, False, False, None),
     (70000, 1, 2, 2, 1, F32, False, True, None),
 ]
 
@@ -405,6 +410,38 @@ def test_selective_scan_extreme_steps(T):
     y = scan_run(p, True, None, out)
     want, err, h, eh = scan_ref(softplus=True, ends=[T], **p)
     assert torch.isfinite(y).all() and torch.isfinite(out).all()
+    _near(y, want, err)
+    _near(out, h, eh)
+
+
+@pytest.mark.parametrize("T", [1, 60, 900])
+def test_selective_scan_keeps_what_is_not_finite_to_its_channel(T):
+    """An infinite step, an infinite or NaN input, a NaN decay: the channel that holds it is not finite from there on, all
+    others are as they were."""
+    p = scan_inputs(1, T, 64, 16, 1, F32, False, True, 12)
+    want = scan_run(p, True, None)
+    q = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in p.items()}
+    at = T // 2
+    q["delta"][0, at, 3], q["u"][0, at, 17], q["u"][0, at, 30], q["A"][45, 2] = float("inf"), float("inf"), float("nan"), float("nan")
+    y = scan_run(q, True, None)
+    bad = [3, 17, 30, 45]
+    good = [d for d in range(64) if d not in bad]
+    assert torch.equal(y[..., good], want[..., good])
+    assert torch.equal(y[:, :at, bad[:3]], want[:, :at, bad[:3]])
+    assert not y[:, at:, bad[:3]].isfinite().any() and y[..., 45].isnan().all()
+
+
+def test_selective_scan_grows_where_its_decays_are_positive():
+    """A > 0 is allowed: a state that starts at zero stays there however far exp(A * sum of dt) overflows, and one that starts
+    late grows as the formula says."""
+    p = scan_inputs(1, 3000, 32, 16, 1, F32, False, False, 13, bias=False)
+    p["A"] = torch.rand(32, 16, generator=_rng(14)) * 0.5
+    p["delta"] = torch.full_like(p["delta"], 0.2)
+    p["u"][:, :2900] = 0
+    out = torch.empty(1, 32, 16, device="cuda")
+    y = scan_run(p, False, None, out)
+    want, err, h, eh = scan_ref(softplus=False, ends=[3000], **p)
+    assert torch.isfinite(y).all() and not y[:, :2900].any()
     _near(y, want, err)
     _near(out, h, eh)
 
@@ -582,6 +619,77 @@ def test_results_do_not_depend_on_the_run_or_the_stream():
             again = work()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@torch.no_grad()
+def test_two_threads_on_two_streams():
+    import threading
+
+    p = scan_inputs(2, 1500, 64, 16, 1, F32, True, True, 75)
+    q = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in p.items()}
+    x = torch.randn(2, 7000, 64, generator=_rng(76)).cuda()
+    work = lambda: (scan_run(q, True, [1500, 900]), sequence.group_norm(x, 4, lengths=[7000, 33]),  # noqa: E731
+                    sequence.causal_conv(x, torch.ones(64, 4, device="cuda"), lengths=[6999, 0]))
+    want, got = work(), [[], []]
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(work())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for g in got for r in g for a, b in zip(r, want)) and len(got[0]) == len(got[1]) == 10
+
+
+# --- far apart -----------------------------------------------------------------------------------------------------
+@torch.no_grad()
+def test_sequences_beyond_32_bit_offsets():
+    """The second of two sequences starts 2^31 + elements behind the first: it equals the call on it alone.  A sequence's
+    statistics are put together from pieces whose number goes by the batch: a thread joins at most 1024 batches of a piece, each
+    with 4 roundings, so the two calls' 1 / sqrt(var) differ by under 1024 * 4 * u / 2 of itself = 1.3e-4 and their means (near
+    zero) by less; with |y| < 6.5 that is under 1e-3, and a step of bfloat16 (2^-7 of the value) where the rounding flips."""
+    T, ch = 1 << 20, 2056
+    x = torch.empty(2, T, ch, dtype=BF16, device="cuda")
+    for i in range(0, T, 1 << 16):
+        x[:, i:i + (1 << 16)].normal_()
+    assert x.stride(0) > 2 ** 31
+    w = torch.randn(ch, 4, generator=_rng(1)).cuda()
+    for f in (lambda v: sequence.group_norm(v, 257, per_frame=True), lambda v: sequence.causal_conv(v, w)):
+        both = f(x)
+        assert torch.equal(both[1:], f(x[1:])) and both[1].any()
+        del both
+    both, alone = sequence.group_norm(x, 8, activation="silu"), sequence.group_norm(x[1:], 8, activation="silu")
+    for i in range(0, T, 1 << 16):
+        a, b = both[1, i:i + (1 << 16)].float(), alone[0, i:i + (1 << 16)].float()
+        assert torch.allclose(a, b, rtol=2 ** -7, atol=1e-3) and a.any()
+    del both, alone
+    maps, A = torch.ones(2, T, 1, dtype=BF16, device="cuda"), -torch.ones(ch, 1, device="cuda")
+    step = torch.full((1, 1, 1), 0.1, dtype=BF16, device="cuda").expand(2, T, ch)
+    short = 3000  # (the whole length frame after frame would take a second: the rest is past the sequences' ends)
+    both = sequence.selective_scan(x, step, A, maps, maps, lengths=[100, short])
+    alone = sequence.selective_scan(x[1:, :short].contiguous(), step[1:, :short], A, maps[1:, :short], maps[1:, :short])
+    assert torch.allclose(both[1:, :short].float(), alone.float(), rtol=2 ** -7, atol=1e-4) and not both[1, short:].any()
+
+
+@torch.no_grad()
+def test_single_frames_however_far_the_next_would_be():
+    """[1][B][C] memory as [B, 1, C]: the stride of the frame axis says nothing, and is larger than rows may lie apart."""
+    B, ch = 40000, 1024
+    x = torch.randn(1, B, ch, device="cuda").to(BF16).transpose(0, 1)
+    assert x.shape == (B, 1, ch) and x.stride(1) > 2 ** 25
+    w = torch.randn(ch, 4, generator=_rng(1)).cuda()
+    c = x.contiguous()
+    assert torch.equal(sequence.group_norm(x, 8, per_frame=True), sequence.group_norm(c, 8, per_frame=True))
+    assert torch.equal(sequence.group_norm(x, 8), sequence.group_norm(c, 8))
+    assert torch.equal(sequence.causal_conv(x, w), sequence.causal_conv(c, w))
+    bc, A = x[..., :4], -torch.ones(ch, 4, device="cuda")
+    assert torch.equal(sequence.selective_scan(x, x, A, bc, bc, z=x), sequence.selective_scan(c, c, A, bc.contiguous(), bc.contiguous(), z=c))
 
 
 # --- the C entry points on their own -------------------------------------------------------------------------------

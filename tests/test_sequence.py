@@ -52,7 +52,13 @@ BAD = [
     (_scan, dict(Bm=None), b"Bm needs"), (_scan, dict(Cm=None), b"Cm needs"), (_scan, dict(z=P + 2), b"z needs"),
     (_scan, dict(y=None), b"output needs"), (_scan, dict(y_batch_stride=0), b"overlap"),
     (_scan, dict(state_out=3 * P + 4), b"overlap"), (_scan, dict(dtype=7), b"dtype"), (_scan, dict(D=0), b"sizes"),
-    (_scan, dict(B=-2), b"sizes"),
+    (_scan, dict(B=-2), b"sizes"), (_scan, dict(Bg_stride=-16), b"strides"), (_scan, dict(Cg_stride=-1), b"strides"),
+    (_scan, dict(A=P + 2), b"aligned"), (_scan, dict(state_in=P + 1, state_out=None), b"aligned"),
+    (_scan, dict(lengths=P + 2), b"aligned"), (_conv, dict(weight=P + 2), b"aligned"), (_conv, dict(bias=P + 3), b"aligned"),
+    (_norm, dict(weight=P + 2), b"aligned"), (_norm, dict(lengths=P + 1), b"aligned"),
+    (_norm, dict(T=2 ** 30 + 1), b"sizes"), (_norm, dict(x_row_stride=2 ** 25 + 1), b"row stride"),
+    (_conv, dict(C=2 ** 27 + 1, K=1), b"channels"), (_scan, dict(D=2 ** 22 + 1), b"channels"),
+    (_scan, dict(B=2 ** 20, D=2 ** 10), b"2^29"),
 ]
 
 
