@@ -1,6 +1,15 @@
 // selective_scan.hip -- the selective state space recurrence on channels-last tensors (mv_selective_scan).
 //
 //   h[n] = exp(dt A[d, n]) h[n] + dt u B[g, n],   y = (sum_n C[g, n] h[n] + D u) z sigmoid(z)
+//
+// What bounds it.  Many frames: the vector unit.  A state costs an exponential (8.6 cycles of a SIMD, measured), the product in
+// its argument and two multiply-adds (2.9 each with two waves on the SIMD, 4 - 5 with one): 17 cycles for 64 states against
+// 8 bytes a channel and frame, so 16 states of 1024 channels take twice what their bytes would.  What is left of the unit goes
+// to the steps' softplus, the gate and the sums over states.  Frames of a channel are a chain: the parallelism is sequences x
+// channels, four lanes to a channel (scan_kernel), and pieces of the frames where that does not fill the chip, at the price of
+// going through them twice (a piece's decay needs no more than its sum of dt: exp(A sum dt)).  32 utterances of 172 - 861
+// frames, 1024 channels, 16 states, bf16: 94 us; one of 8192 frames: 75 us.
+// One frame of many sequences: the state, in and out once (scan_step_kernel).  512 sequences, 71 MB: 17.8 us, 4.0 TB/s.
 #include "sequence.h"
 
 namespace mv {
@@ -538,15 +547,19 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
 
 constexpr int kStepBlocks = 2048;  // of the step kernel: eight to a CU, each then walks B * D / 64 / 2048 sequences
 
-// Calls of up to this many frames take the step kernel.
-constexpr int kStepFrames = 4;
+// Calls of up to this many frames take the step kernel, whose frames cost their own memory instructions; the other one computes
+// 16 at a time (D 1024, 64 / 512 sequences: 8 frames 11.2 / 38.5 us against 14.0 / 91; 16 frames of 64 sequences 17.3 against 14).
+constexpr int kStepFrames = 8;
 
-// Pieces that the frames of each sequence are cut into.
+// Pieces that the frames of each sequence are cut into: as many as give every SIMD two waves (which is what the registers
+// hold), of 32 frames at least.  The work doubles, so two pieces gain nothing (1 x 8192 frames, D 1024: 111 us with waves for
+// one a SIMD, 81 for two, 92 for three or four; 8 x 861: 70 cut in four, 86 whole; 12 x 861: 86 whole, 100 in three), and a
+// launch takes what 30 frames take (1 x 861, D 256: 17.9 us in 27 pieces of 32, 21.7 in 14 of 64).
 static int scan_pieces(int B, int T, int D, int G) {
     const long long waves = (long long)B * G * ((D / G + 15) / 16);
     if (waves >= 1024 || T < 96) return 1;
     long long n = 2048 / waves;
-    n = std::min<long long>(n, T / 32);
+    n = std::min<long long>(n, (T + 31) / 32);
     n = std::min<long long>(n, 128);
     return n < 3 ? 1 : (int)n;
 }
