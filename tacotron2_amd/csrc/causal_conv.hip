@@ -34,7 +34,10 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(CausalParams<T> p) {
     const unsigned id = blockIdx.x * 256 + threadIdx.x, rest = id / p.vecs;
     const int cv = id % p.vecs, r = p.runs == 1 ? 0 : rest % p.runs, b = p.runs == 1 ? rest : rest / p.runs;
     if (b >= p.B) return;
-    const int c = cv * V, n = min(V, p.C - c), len = seq_frames(p.lengths, b, p.Tmax);
+    // The last vector of a row whose channels are no multiple of V reaches back over its neighbour's and writes what that one
+    // writes; where the state is moved on, one thread alone may read a channel's and write it, and it has what is left.
+    const bool back = cv * V + V > p.C && p.C >= V && !(r == 0 && p.state_out);
+    const int c = back ? p.C - V : cv * V, n = min(V, p.C - c), len = seq_frames(p.lengths, b, p.Tmax);
     const int t0 = r * p.run, t1 = min(t0 + p.run, p.Tmax);
     const T* from = p.x.row(b, 0) + c;
     T* to = p.y.row(b, 0) + c;

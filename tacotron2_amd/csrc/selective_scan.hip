@@ -187,8 +187,12 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
     // The next tile on its way: a thread brings one vector of a row of u, delta, z each (256 threads cover a tile) and kMine
     // elements of B and C.  A frame past t1 - 1 is that frame again; nothing reads it but for zeros in its place.  Addresses
     // are a base that all threads share (scalar arithmetic) plus an offset that a thread keeps.
-    const int vrow = tid / Tl::vecs, vcol = tid % Tl::vecs * Tl::vec;
-    const int vn = min(Tl::vec, p.D / p.G - c0 - vcol);  // channels of the vector that the group has
+    const int vrow = tid / Tl::vecs;
+    int vcol = tid % Tl::vecs * Tl::vec, vn = min(Tl::vec, p.D / p.G - c0 - vcol);  // channels of the vector that the group has
+    if (vn > 0 && vn < Tl::vec && vcol >= Tl::vec - vn) {  // reaches back over its neighbour's, which brings the same
+        vcol -= Tl::vec - vn;
+        vn = Tl::vec;
+    }
     const int d0 = ch.g * (p.D / p.G) + c0 + vcol;
     constexpr int kRows = 256 / NP > Tl::frames ? Tl::frames : 256 / NP;  // rows of B and C that the block brings at once
     const int mrow = tid / NP % Tl::frames, mn = min(tid % NP, p.N - 1);

@@ -58,7 +58,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, slo
             bias, wtype, bp = _weight("group_norm", "bias", bias, (ch,), dtype, dev)
     if _grad():
         _no_grad("group_norm", x, weight, bias)
-    y = _like(x) if x.is_contiguous() else _empty(shape, dtype=dtype, device=x.device)
+    y = _like(x, memory_format=_DENSE)
     if B and T:
         if lengths is not None:
             lengths = _lengths(lengths, B, T, x)
@@ -95,7 +95,7 @@ def causal_conv(x, weight, bias=None, activation=None, slope=0.1, state=None, st
         op = _state("causal_conv", "state_out", state_out, (B, K - 1, ch), dtype, dev)
     if _grad():
         _no_grad("causal_conv", x, weight, bias, state, state_out)
-    y = _like(x) if x.is_contiguous() else _empty(shape, dtype=dtype, device=x.device)
+    y = _like(x, memory_format=_DENSE)
     if B and (T or state_out is not None):
         if lengths is not None:
             lengths = _lengths(lengths, B, T, x)
@@ -154,7 +154,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         op = _state("selective_scan", "state_out", state_out, (nb, ch, N), torch.float32, dev)
     if _grad():
         _no_grad("selective_scan", u, delta, z, B, C, A, D, delta_bias, state, state_out)
-    y = _like(u) if u.is_contiguous() else _empty(shape, dtype=dtype, device=u.device)
+    y = _like(u, memory_format=_DENSE)
     if nb and (T or state_out is not None):
         if lengths is not None:
             lengths = _lengths(lengths, nb, T, u)
@@ -170,7 +170,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
 
 # --- arguments.  A decode step's call is short against what Python adds to it: checks are plain comparisons, messages are made
 # --- where one fails.
-_INF, _NO_STRIDES = float("inf"), (0, 0, 0)
+_INF, _NO_STRIDES, _DENSE = float("inf"), (0, 0, 0), torch.contiguous_format
 _empty, _like, _grad = torch.empty, torch.empty_like, torch.is_grad_enabled
 
 
