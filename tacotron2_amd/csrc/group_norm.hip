@@ -12,7 +12,11 @@
 //   group_apply_kernel    put together and x is read a second time
 //   wide_norm_kernel      what none of them holds: groups of more channels than a block holds at once
 //
-// A vector is the largest power of two of channels, 16 bytes at most, that divides a group: it never holds two groups.
+// A vector is as many channels of a group as there are, a power of two of them, 16 bytes at most, at any address.  It never
+// holds two groups: where the group is no multiple of it (R), the group's last vector reaches back over the one before; what
+// both hold counts once (`skip`), and both write the same.  32 x 861 frames, bf16, C about 512: groups of 17 channels 26 us
+// and per frame 24 us (31 and 111 us with the largest vector that divides the group, one channel), of 7 20 and 20 us (59 and
+// 60 us), of 16, where nothing overlaps, 15 and 14 us; a group of one channel, a vector of its own, 78 us.
 #include "sequence.h"
 
 namespace mv {
@@ -103,6 +107,25 @@ __device__ __forceinline__ typename Unaligned<T, V>::type normalise(typename Una
     return y;
 }
 
+// sums over a vector's elements, those from `skip` on where vectors reach back (R)
+template <typename T, int V, bool R>
+__device__ __forceinline__ float sum_of(typename Unaligned<T, V>::type x, int skip) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += !R || e >= skip ? (float)x[e] : 0.f;
+    return s;
+}
+template <typename T, int V, bool R>
+__device__ __forceinline__ float squares_of(typename Unaligned<T, V>::type x, float mean, int skip) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float d = !R || e >= skip ? (float)x[e] - mean : 0.f;
+        s += d * d;
+    }
+    return s;
+}
+
 // A vector as it was loaded, for the compiler a new value: what is computed from it is computed again rather than kept, and
 // the registers that hold a tile hold its 16-bit elements, not their float32 conversions.
 template <typename Vec>
@@ -140,18 +163,23 @@ __device__ __forceinline__ float group_total(float v, float* red, int rows, int 
 
 // A block's thread on a tile of vectors of a row: which vector, which rows (row, row + rows, ...), which group of the tile.
 // Addresses are a base that the block shares plus a 32-bit offset of the thread (the plan sees to it that it fits).
-template <typename T, int V>
+template <typename T, int V, bool R>
 struct Place {
-    int row, rows, c, mine, gv;
-    bool in;  // false: a thread without a row, or past the last vector of a row; it loads what its neighbour does
+    int row, rows, c, skip, mine, gv;
+    bool first;  // of its group
+    bool in;     // false: a thread without a row, or past the last vector of a row; it loads what its neighbour does
 
     __device__ __forceinline__ Place(const NormParams<T>& p, int tile) {
         const int tile0 = tile * p.tile, v = threadIdx.x % p.tile;
-        gv = p.C / p.G / V;
+        const int Cg = p.C / p.G;
+        gv = (Cg + V - 1) / V;
         rows = blockDim.x / p.tile;
         row = min((int)threadIdx.x / p.tile, rows - 1);
-        in = threadIdx.x < rows * p.tile && tile0 + v < p.C / V;
-        c = min(tile0 + v, p.C / V - 1) * V;
+        in = threadIdx.x < rows * p.tile && tile0 + v < p.G * gv;
+        const int at = min(tile0 + v, p.G * gv - 1), k = at % gv;
+        c = R ? at / gv * Cg + min(k * V, Cg - V) : at * V;
+        skip = R && k == gv - 1 ? gv * V - Cg : 0;
+        first = k == 0;
         mine = v / gv;
     }
     // frame t0 + row + i * rows; frames from `end` on: frame end - 1
@@ -165,35 +193,28 @@ struct Place {
 };
 
 // Frames [t0, t1) of a tile in the block's registers, NI vectors to a thread, and the statistics of the thread's group.
-template <typename T, int V, int NI>
+template <typename T, int V, int NI, bool R>
 struct Held {
     typedef typename Unaligned<T, V>::type Vec;
     Vec x[NI];
     float mean, m2;
 
     // count: frames * channels of the group
-    __device__ __forceinline__ void take(const NormParams<T>& p, const Place<T, V>& at, int b, int t0, int t1, float count,
+    __device__ __forceinline__ void take(const NormParams<T>& p, const Place<T, V, R>& at, int b, int t0, int t1, float count,
                                          float* red) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) x[i] = *(const Vec*)at.at(p.x.row(b, 0), p.x.rs, t0, i, t1);
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (at.in && t0 + at.row + i * at.rows < t1)
-#pragma unroll
-                for (int e = 0; e < V; ++e) s += (float)x[i][e];
+            if (at.in && t0 + at.row + i * at.rows < t1) s += sum_of<T, V, R>(x[i], at.skip);
         mean = group_total(s, red, at.rows, p.tile, at.gv, at.mine) / count;
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NI; ++i) x[i] = forget(x[i]);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (at.in && t0 + at.row + i * at.rows < t1)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float d = (float)x[i][e] - mean;
-                    s += d * d;
-                }
+            if (at.in && t0 + at.row + i * at.rows < t1) s += squares_of<T, V, R>(x[i], mean, at.skip);
         m2 = group_total(s, red, at.rows, p.tile, at.gv, at.mine);
 #pragma unroll
         for (int i = 0; i < NI; ++i) x[i] = forget(x[i]);
@@ -204,15 +225,15 @@ constexpr int kNormThreads = 1024;
 
 // One block to a tile of a sequence: whole groups of it, all frames.  Blocks go to the 8 XCDs in turn; here each XCD gets a
 // run of tiles, so that tiles that share a 128-byte line meet in one L2.
-template <typename T, int V, int NI, int ACT>
+template <typename T, int V, int NI, int ACT, bool R>
 __global__ __launch_bounds__(kNormThreads) void group_norm_kernel(NormParams<T> p) {
     __shared__ float red[2 * kNormThreads];
     typedef typename Unaligned<T, V>::type Vec;
     const unsigned work = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int b = work / p.tiles;
     if (b >= p.B) return;
-    const Place<T, V> at(p, work - b * p.tiles);
-    Held<T, V, NI> h;
+    const Place<T, V, R> at(p, work - b * p.tiles);
+    Held<T, V, NI, R> h;
     const int len = seq_frames(p.lengths, b, p.Tmax);
     const float count = (float)len * (float)(p.C / p.G);
     if (len) h.take(p, at, b, 0, len, count, red);
@@ -240,11 +261,11 @@ __global__ __launch_bounds__(kNormThreads) void group_norm_kernel(NormParams<T> 
 // mean' = mean + d n2 / n', m2' = m2 + q + d^2 n n2 / n' with d the distance of the means); the block's threads are put
 // together the same way at the end.
 constexpr int kStatRows = 8;
-template <typename T, int V>
+template <typename T, int V, bool R>
 __global__ __launch_bounds__(kNormThreads) void group_stats_kernel(NormParams<T> p) {
     __shared__ float red[2 * kNormThreads];
     typedef typename Unaligned<T, V>::type Vec;
-    const Place<T, V> at(p, blockIdx.x);
+    const Place<T, V, R> at(p, blockIdx.x);
     const int Cg = p.C / p.G;
     for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
         const int len = seq_frames(p.lengths, b, p.Tmax);
@@ -256,24 +277,17 @@ __global__ __launch_bounds__(kNormThreads) void group_stats_kernel(NormParams<T>
             for (int i = 0; i < kStatRows; ++i) x[i] = *(const Vec*)at.at(p.x.row(b, 0), p.x.rs, t, i, t1);
             // this thread's frames of the batch: t + row, t + row + rows, ...
             const int mine = at.in ? min(kStatRows, max(0, (t1 - t - at.row + at.rows - 1) / at.rows)) : 0;
-            const float n2 = (float)(mine * V);
+            const float n2 = (float)(mine * (V - at.skip));
             if (mine > 0) {
                 float s = 0.f;
 #pragma unroll
                 for (int i = 0; i < kStatRows; ++i)
-                    if (i < mine)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) s += (float)x[i][e];
+                    if (i < mine) s += sum_of<T, V, R>(x[i], at.skip);
                 const float mu = s / n2;
                 float q = 0.f;
 #pragma unroll
                 for (int i = 0; i < kStatRows; ++i)
-                    if (i < mine)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float d = (float)x[i][e] - mu;
-                            q += d * d;
-                        }
+                    if (i < mine) q += squares_of<T, V, R>(x[i], mu, at.skip);
                 const float all = n + n2, d = mu - mean, part = n2 / all;
                 mean += d * part;
                 m2 += q + d * d * n * part;
@@ -286,7 +300,7 @@ __global__ __launch_bounds__(kNormThreads) void group_stats_kernel(NormParams<T>
             m2 = group_total(n > 0.f ? m2 + n * d * d : 0.f, red, at.rows, p.tile, at.gv, at.mine);
             mean = mu;
         }
-        if (at.in && at.row == 0 && at.c % Cg == 0) {
+        if (at.in && at.row == 0 && at.first) {
             const long long i = ((long long)b * p.G + at.c / Cg) * p.pieces + blockIdx.y;
             p.n[i] = count;
             p.mean[i] = mean;
@@ -316,15 +330,15 @@ __device__ __forceinline__ void join_pieces(const float* n, const float* mean, c
 }
 
 // Grid (tiles, pieces, sequences).  `piece` is this launch's own, a multiple of 4 * rows frames.
-template <typename T, int V, int ACT>
+template <typename T, int V, int ACT, bool R>
 __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T> p) {
     __shared__ float stat[2 * kNormThreads];
     typedef typename Unaligned<T, V>::type Vec;
-    const Place<T, V> at(p, blockIdx.x);
+    const Place<T, V, R> at(p, blockIdx.x);
     float w[V], bias[V];
     load_weights<T, V>(p.w, p.w32, at.c, 1.f, w);
     load_weights<T, V>(p.b, p.w32, at.c, 0.f, bias);
-    const int Cg = p.C / p.G, g0 = blockIdx.x * p.tile * V / Cg, groups = p.tile * V / Cg;
+    const int groups = p.tile / at.gv, g0 = blockIdx.x * groups;
     for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
         const int len = seq_frames(p.lengths, b, p.Tmax);
         const int t0 = blockIdx.y * p.piece, te = min(t0 + p.piece, p.Tmax), live = min(te, len);
@@ -361,16 +375,18 @@ __global__ __launch_bounds__(kNormThreads) void group_apply_kernel(NormParams<T>
 
 // Each frame's groups by themselves: L lanes to a group, NI vectors to a lane.  A slot of L lanes keeps its group (and its
 // weights) and walks the frames.
-template <typename T, int V, int NI, int ACT>
+template <typename T, int V, int NI, int ACT, bool R>
 __global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L, unsigned slots) {
     typedef typename Unaligned<T, V>::type Vec;
     const unsigned slot = (blockIdx.x * 256 + threadIdx.x) >> (31 - __builtin_clz(L));
     if (slot >= slots) return;  // (whole slots leave: L divides 64)
-    const int l = threadIdx.x & (L - 1), Cg = p.C / p.G, nv = Cg / V, g = slot % p.G;
+    const int l = threadIdx.x & (L - 1), Cg = p.C / p.G, nv = (Cg + V - 1) / V, g = slot % p.G;
+    auto from_of = [&](int i) { return R ? min((l + i * L) * V, Cg - V) : (l + i * L) * V; };
+    auto skip_of = [&](int i) { return R && l + i * L == nv - 1 ? nv * V - Cg : 0; };
     float w[NI][V], bias[NI][V];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int c = g * Cg + min(l + i * L, nv - 1) * V;
+        const int c = g * Cg + min((l + i * L) * V, Cg - V);
         load_weights<T, V>(p.w, p.w32, c, 1.f, w[i]);
         load_weights<T, V>(p.b, p.w32, c, 0.f, bias[i]);
     }
@@ -384,7 +400,7 @@ __global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L,
                 Vec y;
 #pragma unroll
                 for (int e = 0; e < V; ++e) y[e] = (T)0.f;
-                if (l + i * L < nv) *(Vec*)(to + (l + i * L) * V) = y;
+                if (l + i * L < nv) *(Vec*)(to + from_of(i)) = y;
             }
             continue;
         }
@@ -393,28 +409,21 @@ __global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L,
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (l + i * L < nv) x[i] = *(const Vec*)(from + (l + i * L) * V);
+            if (l + i * L < nv) x[i] = *(const Vec*)(from + from_of(i));
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (l + i * L < nv)
-#pragma unroll
-                for (int e = 0; e < V; ++e) s += (float)x[i][e];
+            if (l + i * L < nv) s += sum_of<T, V, R>(x[i], skip_of(i));
         for (int m = L >> 1; m; m >>= 1) s += __shfl_xor(s, m);
         const float mean = s / (float)Cg;
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (l + i * L < nv)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float d = (float)x[i][e] - mean;
-                    s += d * d;
-                }
+            if (l + i * L < nv) s += squares_of<T, V, R>(x[i], mean, skip_of(i));
         for (int m = L >> 1; m; m >>= 1) s += __shfl_xor(s, m);
         const float rstd = 1.f / sqrtf(s / (float)Cg + p.eps);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (l + i * L < nv) *(Vec*)(to + (l + i * L) * V) = normalise<T, V, ACT>(x[i], mean, rstd, w[i], bias[i], p.slope);
+            if (l + i * L < nv) *(Vec*)(to + from_of(i)) = normalise<T, V, ACT>(x[i], mean, rstd, w[i], bias[i], p.slope);
     }
 }
 
@@ -478,7 +487,7 @@ __global__ __launch_bounds__(256) void wide_norm_kernel(NormParams<T> p, int per
 enum { NORM_FRAME, NORM_HELD, NORM_PIECES, NORM_WIDE };
 struct NormPlan {
     int kind, V, NI, threads, tile, tiles, piece, pieces, apply_piece, L;
-    bool past;
+    bool past, reach;
     size_t bytes;
 };
 
@@ -493,8 +502,12 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     NormPlan s{};
     const int Cg = a->C / a->groups, size = (int)dtype_size(a->dtype);
     s.V = 16 / size;
-    while (Cg % s.V) s.V /= 2;
-    const int gv = Cg / s.V, row = a->C / s.V;
+    while (s.V > Cg) s.V /= 2;
+    // (in place, two vectors that share channels must not be two threads' whose order nothing sets)
+    if (!a->per_frame && a->x.ptr == a->y.ptr)
+        while (Cg % s.V) s.V /= 2;
+    s.reach = Cg % s.V != 0;
+    const int gv = ceil_div(Cg, s.V), row = a->groups * gv;
     s.kind = NORM_WIDE;
     if (a->per_frame) {
         if (gv > 64 * 8) return s;
@@ -516,7 +529,7 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     s.tile = gv;
     s.past = pass_by_l2(a->y, a->B, a->T, a->C, a->dtype);
     grow(s.past ? 64 : 32);
-    s.past = s.past && (s.tile * s.V * size) % 64 == 0;
+    s.past = s.past && !s.reach && (s.tile * s.V * size) % 64 == 0;
     if ((long long)s.tiles * a->B > 4096) grow(128);
     for (s.threads = 64; s.threads <= kNormThreads; s.threads *= 2) {
         if (s.threads < s.tile) continue;
@@ -546,23 +559,24 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// calls f(V, NI) with the plan's vector and count as constants
+// calls f(V, NI, R) with the plan's vector, count and whether vectors reach back as constants
 template <typename T, typename F>
 static int by_plan(const NormPlan& s, F&& f) {
-    auto by_count = [&](auto v) {
+    auto by_count = [&](auto v, auto r) {
         switch (s.NI) {
-            case 1: return f(v, Int<1>());
-            case 2: return f(v, Int<2>());
-            case 4: return f(v, Int<4>());
-            case 8: return f(v, Int<8>());
-            default: return f(v, Int<16>());
+            case 1: return f(v, Int<1>(), r);
+            case 2: return f(v, Int<2>(), r);
+            case 4: return f(v, Int<4>(), r);
+            case 8: return f(v, Int<8>(), r);
+            default: return f(v, Int<16>(), r);
         }
     };
+    auto by_reach = [&](auto v) { return s.reach ? by_count(v, std::true_type()) : by_count(v, std::false_type()); };
     switch (s.V) {
-        case 1: return by_count(Int<1>());
-        case 2: return by_count(Int<2>());
-        case 4: return by_count(Int<4>());
-        default: return by_count(Int<(sizeof(T) == 2 ? 8 : 4)>());
+        case 1: return by_count(Int<1>(), std::false_type());
+        case 2: return by_reach(Int<2>());
+        case 4: return by_reach(Int<4>());
+        default: return by_reach(Int<(sizeof(T) == 2 ? 8 : 4)>());
     }
 }
 
@@ -579,8 +593,9 @@ static int launch_norm(const mv_group_norm_args* a, const NormPlan& s, NormParam
         MV_HIP(hipGetLastError());
         return MV_OK;
     }
-    return by_plan<T>(s, [&](auto v, auto n) {
+    return by_plan<T>(s, [&](auto v, auto n, auto r) {
         constexpr int V = decltype(v)::value, NI = decltype(n)::value;
+        constexpr bool R = decltype(r)::value;
         if (s.kind == NORM_FRAME) {
             if constexpr (NI <= 8) {
                 const long long frames = (long long)a->B * a->T, most = 2048ll * 256 / s.L / a->groups;
@@ -589,22 +604,22 @@ static int launch_norm(const mv_group_norm_args* a, const NormPlan& s, NormParam
                     set_error("mv_group_norm: more than 2^31 frames, or groups of a frame, in one call");
                     return MV_EINVAL;
                 }
-                hipLaunchKernelGGL((frame_norm_kernel<T, V, NI, ACT>), dim3((unsigned)((slots * s.L + 255) / 256)), dim3(256), 0,
+                hipLaunchKernelGGL((frame_norm_kernel<T, V, NI, ACT, R>), dim3((unsigned)((slots * s.L + 255) / 256)), dim3(256), 0,
                                    stream, p, s.L, (unsigned)slots);
             }
         } else if constexpr (NI != 2) {
             p.tile = s.tile;
             p.tiles = s.tiles;
             if (s.kind == NORM_HELD) {
-                hipLaunchKernelGGL((group_norm_kernel<T, V, NI, ACT>), dim3((s.tiles * a->B + 7) / 8 * 8), dim3(s.threads), 0,
+                hipLaunchKernelGGL((group_norm_kernel<T, V, NI, ACT, R>), dim3((s.tiles * a->B + 7) / 8 * 8), dim3(s.threads), 0,
                                    stream, p);
             } else if constexpr (NI == 1) {
                 p.piece = s.piece;
                 p.pieces = s.pieces;
-                hipLaunchKernelGGL((group_stats_kernel<T, V>), dim3(s.tiles, s.pieces, B16), dim3(s.threads), 0, stream, p);
+                hipLaunchKernelGGL((group_stats_kernel<T, V, R>), dim3(s.tiles, s.pieces, B16), dim3(s.threads), 0, stream, p);
                 MV_HIP(hipGetLastError());
                 p.piece = s.apply_piece;
-                hipLaunchKernelGGL((group_apply_kernel<T, V, ACT>), dim3(s.tiles, ceil_div(a->T, s.apply_piece), B16),
+                hipLaunchKernelGGL((group_apply_kernel<T, V, ACT, R>), dim3(s.tiles, ceil_div(a->T, s.apply_piece), B16),
                                    dim3(s.threads), 0, stream, p);
             }
         }

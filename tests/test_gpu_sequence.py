@@ -761,6 +761,40 @@ def test_group_norm_in_place():
         assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("width,G", [(3, 5), (5, 3), (6, 4), (7, 1), (9, 2), (15, 4), (17, 3), (33, 2), (255, 1), (1023, 2)])
+def test_group_norm_widths_that_no_vector_divides(dtype, width, G):
+    """The last vector of a group reaches back: its channels count once, and the neighbouring groups' do not count."""
+    for T, per_frame in ((1, True), (29, True), (29, False), (700, False), (5003 if width < 255 else 1200, False)):
+        g = _rng(width * 31 + T)
+        C = width * G
+        x = (torch.randn(2, T, C, generator=g) + 3 * torch.randn(G, generator=g).repeat_interleave(width)).to(dtype)
+        w, b = 1 + 0.2 * torch.randn(C, generator=g), 0.1 * torch.randn(C, generator=g)
+        ends = [T, (T + 1) // 2]
+        y = sequence.group_norm(x.cuda(), G, w.cuda(), b.cuda(), activation="silu", per_frame=per_frame, lengths=_on(ends))
+        _near(y, *norm_ref(x, G, w, b, 1e-5, "silu", per_frame, ends), what=f"T {T} per_frame {per_frame}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width,G", [(7, 3), (17, 2), (129, 1)])
+def test_group_norm_in_place_of_widths_that_no_vector_divides(dtype, width, G):
+    import ctypes
+
+    for T, per_frame in ((1, 1), (30, 1), (30, 0), (900, 0), (6000, 0)):
+        g = _rng(width + T)
+        C = width * G
+        x = torch.randn(2, T, C, generator=g).to(dtype)
+        y = x.cuda()
+        a = _native.mv_group_norm_args(y.data_ptr(), T * C, C, y.data_ptr(), T * C, C, None, None, None, 2, T, C, G,
+                                       1 if dtype == BF16 else 0, 0, per_frame, 3, 0.1, 1e-5)
+        lib = _native.lib()
+        n = lib.mv_group_norm_workspace(ctypes.byref(a))
+        ws = torch.empty(n + 256, dtype=torch.uint8, device="cuda")
+        assert lib.mv_group_norm(ctypes.byref(a), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        _near(y, *norm_ref(x, G, None, None, 1e-5, "tanh", bool(per_frame), [T, T]), what=f"T {T} per_frame {per_frame}")
+
+
 # --- refusals ------------------------------------------------------------------------------------------------------
 def test_refusals():
     f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
