@@ -263,7 +263,7 @@ typedef struct mv_group_norm_args {
     float slope;        /* of MV_ACT_LRELU */
     float eps;          /* >= 0 */
 } mv_group_norm_args;
-/* scratch of mv_group_norm in bytes (256-byte aligned; 0: none needed, workspace may be NULL; T = 1 never needs any) */
+/* scratch of mv_group_norm with the same arguments in bytes (256-byte aligned; 0: none needed, workspace may be NULL; T = 1 never needs any) */
 MV_API size_t mv_group_norm_workspace(const mv_group_norm_args* a);
 MV_API int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -2,7 +2,10 @@
 //
 //   y[t, c] = act(bias_c + sum_k w[c, k] x[t - K + 1 + k, c]),  frames before the first from the state
 //
-// HBM-bound: x once in, y once out.
+// HBM-bound: x once in, y once out; a few kilobytes are bound by the launch.  A thread holds 16 bytes of adjacent channels (the
+// widest load) and walks along time, so a frame comes in once per run and its K uses are registers; the activation's exponential
+// and reciprocal hide behind the loads.  4 taps, SiLU, bf16: 32 x 861 x 512 16 us (3.5 TB/s), 16 x 8192 x 512 57 us (4.7 TB/s),
+// 4 x 16384 x 4096 202 us (5.3 TB/s; a large copy reaches 5.0).
 #include "sequence.h"
 
 namespace mv {
@@ -195,8 +198,14 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         constexpr int V = 16 / sizeof(T);
         CausalParams<T> p{rows_of<const T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->state_in, (T*)a->state_out,
                         a->lengths, a->B, a->T, a->C, a->weight_dtype == MV_DTYPE_F32, 0.f, (unsigned)(a->C + V - 1) / V, 0, 0, pass_by_l2(a->y, a->B, a->T, a->C, a->dtype)};
-        // long runs read few frames twice (K - 1 a run), short ones give more threads: as long as 2^17 of them allow
-        for (p.run = 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;) p.run /= 2;
+        // A run reads K - 1 frames that the one before reads too: runs of 32 frames, halved (to 8) until there are 2^17
+        // threads (1 x 861 x 512: 8.0 us with runs of 8, 13.7 with 32).  Two taps, or up to four where the frames read twice
+        // are in the block's own cache (up to 16 vectors a row) or weigh little (float32), gain more from threads: runs of 8
+        // (4 taps, runs of 8 / 32: bf16 8 x 30000 x 128 26 / 33 us, float32 16 x 8192 x 512 93 / 103, 2 taps bf16 the same
+        // 48 / 54; but 4 taps bf16 8 x 8192 x 1023 63 / 53, 8 taps float32 16 x 8192 x 512 171 / 143).
+        const bool short_runs = a->K <= 2 || (a->K <= 4 && (sizeof(T) == 4 || p.vecs <= 16));
+        for (p.run = short_runs ? 8 : 32; p.run > 8 && (long long)a->B * ((a->T + p.run - 1) / p.run) * p.vecs < 1 << 17;)
+            p.run /= 2;
         p.runs = (a->T + p.run - 1) / p.run;
         const long long blocks = ((long long)a->B * p.runs * p.vecs + 255) / 256;
         if (blocks > 0x7fffff) {

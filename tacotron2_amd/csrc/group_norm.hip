@@ -520,7 +520,9 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     const long long far = std::max(a->x.row_stride, a->y.row_stride);
     auto fits = [&](long long frames) { return (frames * far + a->C) * size < 1ll << 31; };  // Place's offsets
     // Whole groups side by side.  A tile of a whole sequence: rows of 32 bytes at least, as many blocks as that gives (two
-    // and more to a CU, one loading while another reduces or stores), 128 bytes where there are blocks in plenty.
+    // and more to a CU, one loading while another reduces or stores); rows of 64 bytes where results pass by the L2
+    // (32 x 861 x 512, 32 groups, bf16 14.2 us, with 32 bytes 16.8), full lines where that leaves 384 blocks (float32 19.0 us
+    // against 26.9 with 64 bytes; bf16, 256 blocks, 14.6 against 14.2).
     const int most = std::min(row, kNormThreads);
     auto grow = [&](int bytes) {
         while (s.tile * s.V * size < bytes && s.tile + gv <= most) s.tile += gv;
@@ -529,9 +531,14 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     s.tile = gv;
     s.past = pass_by_l2(a->y, a->B, a->T, a->C, a->dtype);
     grow(s.past ? 64 : 32);
+    if (s.past && (long long)a->C * size / 128 * a->B >= 384) grow(128);
     s.past = s.past && !s.reach && (s.tile * s.V * size) % 64 == 0;
     if ((long long)s.tiles * a->B > 4096) grow(128);
-    for (s.threads = 64; s.threads <= kNormThreads; s.threads *= 2) {
+    // A block computes 1000 vectors in 1.3 us; the second launch of the pieces costs 4.  So fewer blocks than CUs hold up to
+    // 4096 vectors each (bf16: 1 x 2000 x 256, 16 groups, 9.4 us held, 11.9 in pieces; 1 x 4000 14.8 and 11.5; 2 x 8192 24.6
+    // and 12.7), more blocks whatever fits (16 x 2000 x 512, 32 groups, 17.9 held, 21.8 in pieces).
+    const bool few = (long long)s.tiles * a->B < 256;
+    for (s.threads = 64; s.threads <= kNormThreads && !(few && (long long)a->T * s.tile > 4096); s.threads *= 2) {
         if (s.threads < s.tile) continue;
         const int n = ceil_div(a->T, s.threads / s.tile);
         if (n <= (s.threads < kNormThreads ? 8 : 16) && fits(s.threads / s.tile * 16ll) &&
@@ -548,7 +555,10 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     const long long want = std::max(1ll, 2048 / ((long long)s.tiles * a->B));
     s.piece = rows * kStatRows * std::max(1, ceil_div(a->T, want * rows * kStatRows));
     s.pieces = ceil_div(a->T, s.piece);
-    s.apply_piece = rows * 32;
+    // The second pass goes in runs of 4 to 32 rows a thread: long ones put the pieces together less often, short ones give
+    // blocks enough (one sequence of 30000 x 128 float32 24.0 us with runs of 32, 15.2 with 4; 16 of 55104 x 128 bf16 123 and 129).
+    for (s.apply_piece = rows * 32; s.apply_piece > rows * 4 && (long long)s.tiles * a->B * ceil_div(a->T, s.apply_piece) < 2048;)
+        s.apply_piece /= 2;
     if (s.pieces > 65535 || ceil_div(a->T, s.apply_piece) > 65535 || !fits(rows * 16ll)) return s;
     s.kind = NORM_PIECES;
     s.NI = 1;
