@@ -795,6 +795,32 @@ def test_group_norm_in_place_of_widths_that_no_vector_divides(dtype, width, G):
         _near(y, *norm_ref(x, G, None, None, 1e-5, "tanh", bool(per_frame), [T, T]), what=f"T {T} per_frame {per_frame}")
 
 
+@pytest.mark.parametrize("dtype,B,T,C,G", [(F32, 32, 300, 512, 32), (F32, 33, 290, 520, 8), (BF16, 64, 300, 512, 64),
+                                           (F32, 2, 17000, 160, 5)])
+def test_group_norm_of_batches_larger_than_the_caches(dtype, B, T, C, G):
+    g = _rng(C + B)
+    x = torch.randn(B, T, C, generator=g).to(dtype)
+    w, b = 1 + 0.2 * torch.randn(C, generator=g), 0.1 * torch.randn(C, generator=g)
+    ends = [T - i * T // (2 * B) for i in range(B)]
+    y = sequence.group_norm(x.cuda(), G, w.cuda(), b.cuda(), activation="silu", lengths=_on(ends))
+    _near(y, *norm_ref(x, G, w, b, 1e-5, "silu", False, ends))
+
+
+@pytest.mark.parametrize("dtype,B,T,C,K", [(F32, 4, 5000, 1030, 3), (BF16, 6, 30000, 120, 4), (BF16, 8, 4100, 516, 2),
+                                           (F16, 8, 4100, 516, 8)])
+def test_causal_conv_of_batches_larger_than_the_caches(dtype, B, T, C, K):
+    g = _rng(C + K)
+    x = torch.randn(B, T, C, generator=g).to(dtype)
+    w = torch.randn(C, K, generator=g) / K
+    ends = [T - i * T // (2 * B) for i in range(B)]
+    out = torch.empty(B, K - 1, C, dtype=dtype, device="cuda")
+    y = sequence.causal_conv(x.cuda(), w.cuda(), activation="silu", state_out=out, lengths=_on(ends))
+    want, err, state = conv_ref(x, w, None, "silu", None, ends)
+    _near(y, want, err)
+    for i, end in enumerate(ends):
+        assert torch.equal(out[i].cpu(), x[i, end - K + 1:end])
+
+
 # --- refusals ------------------------------------------------------------------------------------------------------
 def test_refusals():
     f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
