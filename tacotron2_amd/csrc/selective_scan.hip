@@ -74,8 +74,18 @@ __device__ __forceinline__ float quad_lane(float v, int k) {
     return k == 0 ? quad<0x00>(v) : k == 1 ? quad<0x55>(v) : k == 2 ? quad<0xAA>(v) : quad<0xFF>(v);
 }
 
-// Lane j's NS of the N values at p, as floats; zeros where it has fewer.
-template <typename T, int NS>
+// Four lanes hold NP = 4 * NS states; where a channel has N < NP, no place from N on may add to the sum over states.  Zeros in it
+// do not see to that: an infinite step or input makes a NaN of them (inf * 0).  scan_step_kernel, which waits for memory, writes
+// their h as 0 in every frame.  scan_kernel has no instruction to spare for that; there these places hold the first states once
+// more (NP <= 2 N, or all of them the one state there is): a copy goes the way of its original, to an infinity or a NaN too, and
+// the C of the two (or four) is half (a quarter), so that together they add what one would.
+__device__ __forceinline__ int state_at(int place, int N) { return place < N ? place : N == 1 ? 0 : place - N; }
+__device__ __forceinline__ float share_of(int place, int N, int NP) {
+    return N == 1 ? 1.f / (float)NP : state_at(place, N) < NP - N ? 0.5f : 1.f;
+}
+
+// Lane j's NS of the N values at p, as floats; where it has fewer, zeros or COPIES.
+template <bool COPIES, typename T, int NS>
 __device__ __forceinline__ void load_my_states(const T* p, int N, int j, float (&v)[NS]) {
     if (N == kLanes * NS) {
         typedef typename Unaligned<T, kRun<NS>>::type V;
@@ -87,7 +97,10 @@ __device__ __forceinline__ void load_my_states(const T* p, int N, int j, float (
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) v[s] = state_of<NS>(j, s) < N ? (float)p[state_of<NS>(j, s)] : 0.f;
+        for (int s = 0; s < NS; ++s) {
+            const int place = state_of<NS>(j, s);
+            v[s] = COPIES ? (float)p[state_at(place, N)] : place < N ? (float)p[place] : 0.f;
+        }
     }
 }
 template <int NS>
@@ -110,19 +123,19 @@ __device__ __forceinline__ void store_my_states(float* p, int N, int j, const fl
 
 // A of channel d for exponentials to base 2.  Clamped to finite: 0 * inf must not make a NaN of a frame past the end, whose dt
 // is 0.
-template <typename T, int NS>
+template <bool COPIES, typename T, int NS>
 __device__ __forceinline__ void load_decays(const ScanParams<T>& p, int d, int j, float (&A2)[NS]) {
-    load_my_states(p.A + (long long)d * p.N, p.N, j, A2);
+    load_my_states<COPIES>(p.A + (long long)d * p.N, p.N, j, A2);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const float a = A2[s] * kLog2e;
         A2[s] = a < -3e38f ? -3e38f : (a > 3e38f ? 3e38f : a);  // (a NaN stays one)
     }
 }
-template <int NS>
+template <bool COPIES, int NS>
 __device__ __forceinline__ void load_state(const float* from, int N, int j, float (&h)[NS]) {
     if (from) {
-        load_my_states(from, N, j, h);
+        load_my_states<COPIES>(from, N, j, h);
     } else {
 #pragma unroll
         for (int s = 0; s < NS; ++s) h[s] = 0.f;
@@ -142,7 +155,7 @@ struct Channel {
         live = c < Dg;
         d = g * Dg + min(c, Dg - 1);
         len = seq_frames(p.lengths, b, p.Tmax);
-        load_decays(p, d, j, A2);
+        load_decays<true>(p, d, j, A2);
     }
 };
 
@@ -195,7 +208,8 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
     }
     const int d0 = ch.g * (p.D / p.G) + c0 + vcol;
     constexpr int kRows = 256 / NP > Tl::frames ? Tl::frames : 256 / NP;  // rows of B and C that the block brings at once
-    const int mrow = tid / NP % Tl::frames, mn = min(tid % NP, p.N - 1);
+    const int mrow = tid / NP % Tl::frames, mn = state_at(tid % NP, p.N);
+    const float share = share_of(tid % NP, p.N, NP);
     const long long Bg = ch.g * p.Bg, Cg = ch.g * p.Cg;
     Vec nv[3];
     T nb[kMine], nc[kMine];
@@ -222,12 +236,12 @@ __device__ __forceinline__ float scan_frames(const ScanParams<T>& p, const Chann
         *(Vec*)&to.rows[0][vrow][vcol] = nv[0];
         *(Vec*)&to.rows[1][vrow][vcol] = nv[1];
         if (gate) *(Vec*)&to.rows[2][vrow][vcol] = nv[2];
-        const bool whole = p.N == NP && t + Tl::frames <= t1;
+        const bool whole = t + Tl::frames <= t1;
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int e = tid + 256 * i;
-            float vb = (float)nb[i], vc = Y ? (float)nc[i] : 0.f;
-            if (!whole && !(e % NP < p.N && t + e / NP < t1)) vb = vc = 0.f;
+            float vb = (float)nb[i], vc = Y ? (float)nc[i] * share : 0.f;
+            if (!whole && t + e / NP >= t1) vb = vc = 0.f;
             if (256 * (i + 1) <= Tl::frames * NP || e < Tl::frames * NP) {
                 to.maps[0][0][e] = vb;
                 if (Y) to.maps[1][0][e] = vc;
@@ -436,16 +450,16 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
             }
         } else if (FIRST || t0 < ch.len) {
             if (FIRST) {
-                load_state(p.state_in ? p.state_in + ((long long)b * p.D + ch.d) * p.N : nullptr, p.N, ch.j, h);
+                load_state<true>(p.state_in ? p.state_in + ((long long)b * p.D + ch.d) * p.N : nullptr, p.N, ch.j, h);
             } else {
-                load_my_states(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
+                load_my_states<false>(piece_states(p, ch, 0), kLanes * NS, ch.j, h);
                 constexpr int kBatch = NS >= 16 ? 2 : 8;  // pieces whose loads are in flight together
                 for (int k = 1; k < piece; k += kBatch) {
                     float sum[kBatch], end[kBatch][NS];
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         const int at = min(k + i, piece - 1);
-                        load_my_states(piece_states(p, ch, at), kLanes * NS, ch.j, end[i]);
+                        load_my_states<false>(piece_states(p, ch, at), kLanes * NS, ch.j, end[i]);
                         sum[i] = *piece_sum(p, ch, at);
                     }
 #pragma unroll
@@ -498,7 +512,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
     for (int k = 0; k < Q; ++k) {
         dk[k] = min(c0 + k, p.D - 1);
         gk[k] = p.G == 1 ? 0 : dk[k] / Dg;
-        load_decays(p, dk[k], j, A2[k]);
+        load_decays<false>(p, dk[k], j, A2[k]);
     }
     const float bias = p.bias ? p.bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
     for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
@@ -506,7 +520,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
         const long long state = (long long)b * p.D * p.N;
         float h[Q][NS];
 #pragma unroll
-        for (int k = 0; k < Q; ++k) load_state(p.state_in ? p.state_in + state + dk[k] * p.N : nullptr, p.N, j, h[k]);
+        for (int k = 0; k < Q; ++k) load_state<false>(p.state_in ? p.state_in + state + dk[k] * p.N : nullptr, p.N, j, h[k]);
         for (int t = 0; t < p.Tmax; ++t) {
             float v = 0.f;
             if (t < len) {
@@ -514,8 +528,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
                 const float z = p.z.p ? (float)p.z.row(b, t)[d] : 0.f;
                 float bn[NS], cn[NS], out[Q];
                 auto maps = [&](int k) {
-                    load_my_states(p.Bm.row(b, t) + gk[k] * p.Bg, p.N, j, bn);
-                    load_my_states(p.Cm.row(b, t) + gk[k] * p.Cg, p.N, j, cn);
+                    load_my_states<false>(p.Bm.row(b, t) + gk[k] * p.Bg, p.N, j, bn);
+                    load_my_states<false>(p.Cm.row(b, t) + gk[k] * p.Cg, p.N, j, cn);
                 };
                 maps(0);
                 const float dt = p.softplus ? softplusf(raw) : raw, x = dt * u;
@@ -526,7 +540,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
                     out[k] = 0.f;
 #pragma unroll
                     for (int s = 0; s < NS; ++s) {
-                        h[k][s] = __builtin_fmaf(__builtin_amdgcn_exp2f(dtk * A2[k][s]), h[k][s], xk * bn[s]);
+                        const float hn = __builtin_fmaf(__builtin_amdgcn_exp2f(dtk * A2[k][s]), h[k][s], xk * bn[s]);
+                        h[k][s] = state_of<NS>(j, s) < p.N ? hn : 0.f;
                         out[k] += cn[s] * h[k][s];
                     }
                 }

@@ -861,3 +861,23 @@ def test_refusals():
     long = torch.tensor([2 ** 32 + 1, -2 ** 40], device="cuda")
     assert torch.equal(norm(torch.ones(2, 5, 8, device="cuda"), 2, bias=torch.ones(8, device="cuda"), lengths=long)[:, :, 0],
                        torch.tensor([[1.0] * 5, [0.0] * 5], device="cuda"))
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 5, 12, 16, 20, 33])
+@pytest.mark.parametrize("T,at", [(1, 0), (6, 2), (60, 21), (900, 893)])
+def test_selective_scan_with_any_number_of_states_passes_an_infinity_on(N, T, at):
+    """An infinite step or an infinite input where u, B, C and the states are positive: every state of the channel and y are
+    +inf from that frame on (exp(-inf) h = 0 and inf u B = inf, then a inf = inf), and no NaN comes of lanes without a state."""
+    p = scan_inputs(1, T, 32, N, 1, F32, False, True, 90 + N)
+    for k in ("u", "Bm", "Cm", "state"):
+        p[k] = p[k].abs() + 0.1
+    p["delta"][0, at, 3] = p["u"][0, at, 17] = float("inf")
+    out = torch.empty(1, 32, N, device="cuda")
+    y = scan_run(p, True, None, out)
+    for d in (3, 17):
+        assert (y[0, at:, d] == float("inf")).all() and (out[0, d] == float("inf")).all(), (d, y[0, at:, d], out[0, d])
+    want, err, h, eh = scan_ref(softplus=True, ends=[T], **p)
+    rest = [d for d in range(32) if d not in (3, 17)]
+    _near(y[..., rest], want[..., rest], err[..., rest])
+    _near(y[:, :at], want[:, :at], err[:, :at])
+    _near(out[:, rest], h[:, rest], eh[:, rest])
