@@ -418,6 +418,16 @@ __device__ __forceinline__ int place_to_sequence(const int32_t* lengths, int B, 
     return __builtin_amdgcn_readfirstlane(*found);
 }
 
+// A state after frames whose decays multiply to 2^e, none of them 0 where e is finite: zero and infinities stay what they are
+// however far the factor by itself overflows or underflows, and what the product can hold goes through two halves that float32
+// can hold too.
+__device__ __forceinline__ float decayed(float h, float e) {
+    constexpr int kZero = 0x060, kInf = 0x204, kFinite = 0x1f8;  // classes of both signs
+    const float half = __builtin_amdgcn_exp2f(0.5f * e);
+    const int kept = __builtin_amdgcn_classf(e, kFinite) ? kZero | kInf : kZero;
+    return __builtin_amdgcn_classf(h, kept) ? h : h * half * half;
+}
+
 // Grid (channel blocks of all groups, pieces, sequences).  FIRST: piece 0 from the given state, results and all; every other
 // piece but the last from a zero state, for the state it leaves behind.  Second launch: the pieces from 1 on, each from the
 // state before it, which it puts together from what the first launch left.
@@ -466,8 +476,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
                     for (int i = 0; i < kBatch; ++i)
                         if (k + i < piece)
 #pragma unroll
-                            for (int s = 0; s < NS; ++s)  // (a state of zero stays zero whatever its factor overflows to)
-                                h[s] = (h[s] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sum[i] * ch.A2[s]) * h[s]) + end[i][s];
+                            for (int s = 0; s < NS; ++s) h[s] = decayed(h[s], sum[i] * ch.A2[s]) + end[i][s];
                 }
             }
             if (t0 < t1) scan_frames<T, NS, true>(p, ch, c0, t0, t1, h, lds, steps);

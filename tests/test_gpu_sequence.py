@@ -881,3 +881,38 @@ def test_selective_scan_with_any_number_of_states_passes_an_infinity_on(N, T, at
     _near(y[..., rest], want[..., rest], err[..., rest])
     _near(y[:, :at], want[:, :at], err[:, :at])
     _near(out[:, rest], h[:, rest], eh[:, rest])
+
+
+@pytest.mark.parametrize("N", [5, 16])
+def test_selective_scan_carries_states_over_the_whole_range_of_float32(N):
+    """Steps of both signs, without softplus: the state grows by e^96 and shrinks back within runs of 32 frames, between 1e-30
+    and 5e11.  A factor of a run by itself is no float32 (e^96 > 3.4e38 and e^-96 < 1.2e-38); every value of the state is."""
+    T = 960
+    p = scan_inputs(1, T, 32, N, 1, F32, False, True, 95, bias=False)
+    p["A"], p["D"], p["u"] = torch.full((32, N), -0.5), None, torch.zeros(1, T, 32)
+    p["state"] = 1e-30 * (1 + torch.rand(1, 32, N, generator=_rng(96)))
+    p["Cm"] = p["Cm"].abs() + 0.1
+    p["delta"] = torch.where(torch.arange(T) // 32 % 2 == 0, -6.0, 6.0).view(1, T, 1).expand(1, T, 32).contiguous()
+    out = torch.empty(1, 32, N, device="cuda")
+    y = scan_run(p, False, None, out)
+    want, err, h, eh = scan_ref(softplus=False, ends=[T], **p)
+    assert float((err / want.abs()).max()) < 0.02  # (82 u a frame: the bound says something)
+    _near(y, want, err)
+    _near(out, h, eh)
+
+
+def test_selective_scan_an_infinite_state_outlasts_every_finite_step():
+    """a inf = inf in each frame (a = e^-16 at least), so it is over any run of them, however small the run's factor."""
+    T, at = 900, 100
+    p = scan_inputs(1, T, 32, 16, 1, F32, False, True, 97, bias=False)
+    for k in ("u", "Bm", "Cm", "state"):
+        p[k] = p[k].abs() + 0.1
+    p["A"], p["delta"] = -torch.arange(1, 17).float().expand(32, 16).contiguous(), torch.ones(1, T, 32)
+    p["u"][0, at, 7] = float("inf")
+    out = torch.empty(1, 32, 16, device="cuda")
+    y = scan_run(p, False, None, out)
+    assert (y[0, at:, 7] == float("inf")).all() and (out[0, 7] == float("inf")).all()
+    want, err, h, eh = scan_ref(softplus=False, ends=[T], **p)
+    rest = [d for d in range(32) if d != 7]
+    _near(y[..., rest], want[..., rest], err[..., rest])
+    _near(out[:, rest], h[:, rest], eh[:, rest])
