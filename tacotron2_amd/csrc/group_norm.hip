@@ -511,15 +511,16 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
     s.reach = Cg % s.V != 0;
     const int gv = ceil_div(Cg, s.V), row = a->groups * gv;
     s.kind = NORM_WIDE;
-    if (a->per_frame) {
+    auto by_frame = [&] {
         if (gv > 64 * 8) return s;
         s.kind = NORM_FRAME;
         s.L = pow2_at_least(gv, 64);
         s.NI = pow2_at_least(ceil_div(gv, s.L), 8);
         return s;
-    }
+    };
+    if (a->per_frame) return by_frame();
     if (gv > kNormThreads) return s;
-    const long long far = std::max(a->x.row_stride, a->y.row_stride);
+    const long long far = a->T > 1 ? std::max(a->x.row_stride, a->y.row_stride) : 0;  // (of a single row the stride says nothing)
     auto fits = [&](long long frames) { return (frames * far + a->C) * size < 1ll << 31; };  // Place's offsets
     // Whole groups side by side.  A tile of a whole sequence: rows of 32 bytes at least, as many blocks as that gives (two
     // and more to a CU, one loading while another reduces or stores); rows of 64 bytes where results pass by the L2
@@ -550,6 +551,8 @@ static NormPlan norm_plan(const mv_group_norm_args* a) {
             return s;
         }
     }
+    // a sequence of one frame is that frame: more of them than a grid holds tiles need no pieces and no scratch
+    if (a->T == 1) return s.past = false, by_frame();
     // Pieces: full lines, and enough of them for eight blocks to a CU (padded ones leave at once).
     grow(128);
     s.threads = std::max(256, pow2_at_least(s.tile, kNormThreads));
@@ -598,7 +601,7 @@ static int launch_norm(const mv_group_norm_args* a, const NormPlan& s, NormParam
     if (s.kind == NORM_WIDE) {
         const long long items = (long long)a->B * a->groups * (a->per_frame ? a->T : 1);
         if (items > 0xffffff) {
-            set_error("mv_group_norm: more than 2^24 groups of over %d channels", a->per_frame ? 512 * s.V : kNormThreads * s.V);
+            set_error("mv_group_norm: more than 2^24 groups of over %d channels", a->per_frame || a->T == 1 ? 512 * s.V : kNormThreads * s.V);
             return MV_EINVAL;
         }
         hipLaunchKernelGGL((wide_norm_kernel<T, ACT>), dim3((unsigned)items), dim3(256), 0, stream, p, a->per_frame);

@@ -916,3 +916,18 @@ def test_selective_scan_an_infinite_state_outlasts_every_finite_step():
     rest = [d for d in range(32) if d != 7]
     _near(y[..., rest], want[..., rest], err[..., rest])
     _near(out[:, rest], h[:, rest], eh[:, rest])
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("dtype,C,G", [(BF16, 8, 1), (F32, 4, 2)])
+def test_group_norm_of_more_single_frames_than_a_grid_holds_tiles(dtype, C, G):
+    B, n = 1 << 25, 500
+    x = torch.empty(B, 1, C, dtype=dtype, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    lens = torch.ones(B, dtype=torch.int32, device="cuda")
+    lens[::3] = 0
+    for lengths in (None, lens):
+        y = sequence.group_norm(x, G, activation="silu", lengths=lengths)
+        for part in (slice(0, n), slice(B // 2, B // 2 + n), slice(B - n, B)):
+            ends = [1] * n if lengths is None else lens[part].tolist()
+            _near(y[part], *norm_ref(x[part].cpu(), G, None, None, 1e-5, "silu", False, ends))
+        assert torch.equal(y, sequence.group_norm(x, G, activation="silu", per_frame=True, lengths=lengths))

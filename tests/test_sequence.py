@@ -88,3 +88,20 @@ def test_there_is_no_cpu_path():
         sequence.causal_conv(x, torch.zeros(8, 4))
     with pytest.raises(RuntimeError, match="MI355X only"):
         sequence.selective_scan(x, x, torch.zeros(8, 4), torch.zeros(2, 5, 4), torch.zeros(2, 5, 4))
+
+
+def test_single_frames_never_need_scratch():
+    """What the header promises and the Python layer relies on, up to batches that no grid of whole tiles holds."""
+    lib = _native.lib()
+    for dtype, C, G in ((1, 8, 1), (0, 4, 2), (2, 1, 1), (1, 1024, 1024), (0, 1024, 8), (1, 4096, 1), (0, 20000, 4), (1, 1 << 20, 2)):
+        for B in (1, 3, 1 << 12, 1 << 16, 1 << 20, 1 << 21, 1 << 25, 1 << 28):
+            for per_frame in (0, 1):
+                for far in (C, 1 << 40):  # (of a single row its stride says nothing)
+                    a = _native.mv_group_norm_args(P, C, far, 2 * P, C, far, None, None, None, B, 1, C, G, dtype, 0, per_frame,
+                                                   0, 0.0, 1e-5)
+                    assert lib.mv_group_norm_workspace(ctypes.byref(a)) == 0, (dtype, C, G, B, per_frame, far)
+    for D, N in ((64, 16), (1024, 64)):
+        for B in (1, 1 << 12, 1 << 19):
+            a = _native.mv_selective_scan_args(P, D, D, P, D, D, None, 0, 0, P, N, N, P, N, N, 0, 0, 2 * P, D, D, P, None, None,
+                                               None, None, None, B, 1, D, N, 1, 1, 1)
+            assert lib.mv_selective_scan_workspace(ctypes.byref(a)) == 0
