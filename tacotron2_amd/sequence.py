@@ -20,11 +20,13 @@ stands after its last true frame; they may be the same tensor, so a sequence cut
 gives the results of one call: the convolution bit for bit, the scan to float32 rounding.  Calls can be captured into HIP
 graphs; a decode step on static tensors with its state replaced in place is one kernel.
 
-These are synthesis-time layers: inputs that require a gradient are refused (outside `no_grad`).
+These are synthesis-time layers: inputs that require a gradient are refused (outside `no_grad`), and so are those with a
+forward-mode tangent.
 """
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _native
 
@@ -56,7 +58,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, slo
             weight, wtype, wp = _weight("group_norm", "weight", weight, (ch,), dtype, dev)
         if bias is not None:
             bias, wtype, bp = _weight("group_norm", "bias", bias, (ch,), dtype, dev)
-    if _grad():
+    if _grad() or _forward_ad._current_level >= 0:
         _no_grad("group_norm", x, weight, bias)
     y = _like(x, memory_format=_DENSE)
     if B and T:
@@ -93,7 +95,7 @@ def causal_conv(x, weight, bias=None, activation=None, slope=0.1, state=None, st
         op = sp
     elif state_out is not None:
         op = _state("causal_conv", "state_out", state_out, (B, K - 1, ch), dtype, dev)
-    if _grad():
+    if _grad() or _forward_ad._current_level >= 0:
         _no_grad("causal_conv", x, weight, bias, state, state_out)
     y = _like(x, memory_format=_DENSE)
     if B and (T or state_out is not None):
@@ -152,7 +154,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         op = sp
     elif state_out is not None:
         op = _state("selective_scan", "state_out", state_out, (nb, ch, N), torch.float32, dev)
-    if _grad():
+    if _grad() or _forward_ad._current_level >= 0:
         _no_grad("selective_scan", u, delta, z, B, C, A, D, delta_bias, state, state_out)
     y = _like(u, memory_format=_DENSE)
     if nb and (T or state_out is not None):
@@ -246,9 +248,11 @@ def _state(who, name, t, shape, dtype, dev):
 
 
 def _no_grad(who, *tensors):
+    reverse, forward = _grad(), _forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
     for t in tensors:
-        if t is not None and t.requires_grad:
-            raise RuntimeError(f"tacotron2_amd.sequence.{who} has no gradient: call it under torch.no_grad()")
+        if t is not None and (reverse and t.requires_grad or forward and _forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(f"tacotron2_amd.sequence.{who} has no gradient: call it under torch.no_grad(), without "
+                               "forward-mode tangents")
 
 
 def _lengths(lengths, B, T, x):

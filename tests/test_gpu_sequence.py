@@ -931,3 +931,38 @@ def test_group_norm_of_more_single_frames_than_a_grid_holds_tiles(dtype, C, G):
             ends = [1] * n if lengths is None else lens[part].tolist()
             _near(y[part], *norm_ref(x[part].cpu(), G, None, None, 1e-5, "silu", False, ends))
         assert torch.equal(y, sequence.group_norm(x, G, activation="silu", per_frame=True, lengths=lengths))
+
+
+def test_forward_mode_derivatives_are_refused_like_those_of_reverse_mode():
+    import torch.autograd.forward_ad as fw
+
+    f = lambda *s: torch.ones(*s, device="cuda")  # noqa: E731
+    x, w, A, bc, h, s = f(2, 5, 8), f(8, 4), -f(8, 4), f(2, 5, 4), f(2, 8, 4), f(2, 3, 8)
+    norm, conv, scan = sequence.group_norm, sequence.causal_conv, sequence.selective_scan
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [
+            lambda: norm(dual(x), 2), lambda: norm(x, 2, weight=dual(f(8))), lambda: norm(x, 2, bias=dual(f(8))),
+            lambda: norm(dual(f(2, 8, 5)).transpose(1, 2), 2), lambda: norm(dual(f(2, 8)), 2, per_frame=True),
+            lambda: conv(dual(x), w), lambda: conv(x, dual(w)), lambda: conv(x, w, bias=dual(f(8))),
+            lambda: conv(x, w, state=dual(s)), lambda: scan(dual(x), x, A, bc, bc), lambda: scan(x, dual(x), A, bc, bc),
+            lambda: scan(x, x, dual(A), bc, bc), lambda: scan(x, x, dual(A.half()), bc, bc), lambda: scan(x, x, A, dual(bc), bc),
+            lambda: scan(x, x, A, bc, dual(bc)), lambda: scan(x, x, A, bc, bc, D=dual(f(8))),
+            lambda: scan(x, x, A, bc, bc, z=dual(x)), lambda: scan(x, x, A, bc, bc, delta_bias=dual(f(8))),
+            lambda: scan(x, x, A, bc, bc, state=dual(h)),
+        ]
+        for i, call in enumerate(calls):
+            for _ in range(2):
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call()
+                    pytest.fail(f"call {i} was not refused")
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                    call()  # (no_grad does not switch forward mode off)
+        want = norm(x, 2)  # tensors without a tangent are served as ever
+        d = dual(x)
+        with torch.inference_mode():  # (this does)
+            assert torch.equal(norm(d, 2), want)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: norm(t, 2), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: norm(t, 2))(x[None])
