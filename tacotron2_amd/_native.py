@@ -358,15 +358,17 @@ def workspace(cache: dict, dev, nbytes: int):
 def device_lengths(lengths, B, T, dev):
     """int32 [B] frame counts on `dev`.  Host-side lengths are checked here; lengths that already live on the device
     go through as they are (a check would cost a device->host sync in every call): every kernel of the library
-    clamps the entries it reads into [0, T]."""
+    clamps the entries it reads into [0, T].  Counts of other types are looked at before they become 32 bits."""
     import torch
 
     lengths = torch.as_tensor(lengths)
     if lengths.numel() != B:
         raise RuntimeError("lengths must hold B frame counts in [0, T]")
     if lengths.is_cuda:
+        if lengths.dtype != torch.int32:
+            lengths = (lengths if lengths.is_floating_point() else lengths.long()).clamp(0, T)
         return lengths.to(device=dev, dtype=torch.int32).contiguous()
-    lengths = lengths.to(torch.int32)
+    lengths = lengths.long()
     if B and (int(lengths.max()) > T or int(lengths.min()) < 0):
         raise RuntimeError("lengths must hold B frame counts in [0, T]")
-    return lengths.to(dev, non_blocking=True).contiguous()
+    return lengths.to(torch.int32).to(dev, non_blocking=True).contiguous()

@@ -256,13 +256,14 @@ def _no_grad(who, *tensors):
 
 
 def _lengths(lengths, B, T, x):
-    if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
-        if lengths.numel() != B or lengths.is_floating_point():
-            raise RuntimeError("lengths must hold B frame counts in [0, T]")
-        if lengths.dtype != torch.int32:
-            lengths = lengths.clamp(0, T)  # (a 64-bit count must not wrap around in 32)
-        elif lengths.get_device() == x.get_device() and lengths.is_contiguous():
-            return lengths
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.as_tensor(lengths)
+    if lengths.numel() != B:
+        raise RuntimeError("lengths must hold B frame counts in [0, T]")
+    if lengths.dtype == torch.int32 and lengths.get_device() == x.get_device() and lengths.is_contiguous():
+        return lengths
+    if lengths.is_floating_point() or lengths.is_complex():
+        raise RuntimeError("lengths must be whole numbers")
     return _native.device_lengths(lengths, B, T, x.device)
 
 

@@ -966,3 +966,23 @@ def test_forward_mode_derivatives_are_refused_like_those_of_reverse_mode():
         torch.func.jvp(lambda t: norm(t, 2), (x,), (x,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda t: norm(t, 2))(x[None])
+
+
+def test_lengths_of_every_whole_type():
+    """Counts of a narrower type than the frame count needs, of a wider one, on the device and on the host."""
+    for T, values, types in ((861, [200, 100], (torch.uint8,)), (861, [127, -5], (torch.int8,)),
+                             (55104, [32767, 9], (torch.int16, torch.int64)), (9, [9, 4], (torch.int32, torch.int64, torch.uint8)),
+                             (9, [2 ** 32 + 3, -2 ** 40], (torch.int64,))):
+        x = torch.randn(2, T, 8, device="cuda")
+        want = sequence.group_norm(x, 2, lengths=[min(max(v, 0), T) for v in values])
+        for t in types:
+            lens = torch.tensor(values, dtype=t, device="cuda")
+            assert torch.equal(sequence.group_norm(x, 2, lengths=lens), want), (T, values, t)
+            assert _native.device_lengths(lens, 2, T, x.device).tolist() == [min(max(v, 0), T) for v in values]
+    x = torch.randn(2, 9, 8, device="cuda")
+    for bad in ([2 ** 32 + 3, 1], torch.tensor([2 ** 33, 1]), [5.0, 3.0], torch.tensor([5.5, 3.0]), [float("nan"), 1.0],
+                torch.tensor([5.0, 3.0], device="cuda"), torch.tensor([5 + 0j, 3], device="cuda")):
+        for call in (lambda n: sequence.group_norm(x, 2, lengths=n), lambda n: sequence.causal_conv(x, x[0, :8, :4], lengths=n),
+                     lambda n: sequence.selective_scan(x, x, -x[0, :8, :4].abs(), x[..., :4], x[..., :4], lengths=n)):
+            with pytest.raises(RuntimeError, match="lengths"):
+                call(bad)

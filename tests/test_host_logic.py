@@ -335,3 +335,17 @@ def test_host_side_of_eight_ranks_on_the_configs3_corpus():
     assert rates[1][0] >= 3000.0
     if (os.cpu_count() or 1) >= 8:  # (with fewer cores than ranks the processes time-share)
         assert rates[8][0] >= 1500.0
+
+
+def test_device_lengths_are_looked_at_before_they_become_32_bit():
+    import torch
+
+    from tacotron2_amd import _native
+
+    cpu = torch.device("cpu")
+    for bad in ([2 ** 32 + 3, 1], torch.tensor([1, 2 ** 32]), torch.tensor([1, -2 ** 32 + 1]), np.array([2 ** 40, 0])):
+        with pytest.raises(RuntimeError):
+            _native.device_lengths(bad, 2, 7, cpu)
+    for ok in (np.array([3, 7]), torch.tensor([3, 7], dtype=torch.uint8), torch.tensor([3.0, 7.0]), (3, 7)):
+        got = _native.device_lengths(ok, 2, 7, cpu)
+        assert got.dtype == torch.int32 and got.tolist() == [3, 7]
