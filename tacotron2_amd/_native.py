@@ -368,6 +368,10 @@ def device_lengths(lengths, B, T, dev):
         if lengths.dtype != torch.int32:
             lengths = (lengths if lengths.is_floating_point() else lengths.long()).clamp(0, T)
         return lengths.to(device=dev, dtype=torch.int32).contiguous()
+    if torch.device(dev).type == "cuda":
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():  # the graph would keep the address of memory that is gone at replay
+                raise RuntimeError("lengths must be on the device in a graph capture")
     lengths = lengths.long()
     if B and (int(lengths.max()) > T or int(lengths.min()) < 0):
         raise RuntimeError("lengths must hold B frame counts in [0, T]")

@@ -986,3 +986,22 @@ def test_lengths_of_every_whole_type():
                      lambda n: sequence.selective_scan(x, x, -x[0, :8, :4].abs(), x[..., :4], x[..., :4], lengths=n)):
             with pytest.raises(RuntimeError, match="lengths"):
                 call(bad)
+
+
+@torch.no_grad()
+def test_lengths_of_the_host_are_refused_in_a_capture():
+    """The copy to the device would be recorded with the address of memory that is gone by the time of a replay."""
+    x = torch.randn(2, 9, 8, device="cuda")
+    want, lens = sequence.group_norm(x, 2, lengths=[9, 4]), _on([9, 4])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sequence.group_norm(x, 2)
+        for call in (lambda: sequence.group_norm(x, 2, lengths=[9, 4]), lambda: sequence.causal_conv(x, x[0, :8, :4], lengths=[9, 4])):
+            with pytest.raises(RuntimeError, match="capture"):
+                call()
+        out = sequence.group_norm(x, 2, lengths=lens)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
