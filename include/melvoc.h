@@ -231,7 +231,8 @@ MV_API int mv_pcm16(const float* wav, size_t n, int16_t* pcm, void* stream);
  * device int32 [B] of true frame counts or NULL (all T); entries are clamped into [0, T] by the kernels.  Frames at or past
  * a sequence's end are never read into a result and are written as 0.  Calls run on the current HIP device, are
  * asynchronous on `stream`, allocate nothing and may be captured; the caller owns every buffer.  Outputs must not overlap
- * inputs except where an entry says so.  B = 0 or T = 0 is a call with nothing to do. */
+ * inputs except where an entry says so: refused (MV_EINVAL) where both lie in rows of the same strides, where one of them has
+ * no gaps, or where both start alike; rows laced into rows of other strides are not looked at.  B = 0 or T = 0 is a call with nothing to do. */
 #define MV_DTYPE_F32 0
 #define MV_DTYPE_BF16 1
 #define MV_DTYPE_F16 2

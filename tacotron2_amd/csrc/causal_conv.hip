@@ -193,6 +193,10 @@ extern "C" int mv_causal_conv(const mv_causal_conv_args* a, void* stream) {
         });
     if (int rc = check_rows(who, "x", a->x, a->T, a->dtype)) return rc;
     if (int rc = check_output_rows(who, a->y, a->B, a->T, a->C, a->dtype)) return rc;
+    const Span x(a->x, a->C, a->B, a->T, a->dtype), w(a->weight, (long long)a->C * a->K * wsize), bias(a->bias, a->C * (long long)wsize),
+        lengths(a->lengths, 4ll * a->B), before(a->state_in, states * (long long)size), after(a->state_out, states * (long long)size);
+    if (int rc = check_overlaps(who, Span(a->y, a->C, a->B, a->T, a->dtype), "y", {x, w, bias, lengths, before, after})) return rc;
+    if (int rc = check_overlaps(who, after, "state_out", {x, w, bias, lengths})) return rc;
     return by_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);

@@ -70,6 +70,51 @@ int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, in
     return MV_OK;
 }
 
+// some i in [i0, i1], k in [k0, k1] with lo < d + i * p + k * q < hi (p, q >= 0)
+static bool hits(long long lo, long long hi, long long d, long long i0, long long i1, long long p, long long k0, long long k1,
+                 long long q) {
+    if (i1 - i0 > k1 - k0) std::swap(i0, k0), std::swap(i1, k1), std::swap(p, q);
+    for (long long i = i0; i <= (p ? i1 : i0); ++i) {
+        const long long r = d + i * p;
+        long long k = k0;
+        if (q) {  // the first k past lo
+            const long long n = lo - r, below = n / q - (n % q < 0);
+            k = std::max(k0, below + 1);
+        }
+        if (k <= k1 && r + k * q > lo && r + k * q < hi) return true;
+    }
+    return false;
+}
+
+// Whether two pieces of memory have a byte in common, as far as that is decided: of rows with the same strides (halves of one
+// buffer), of rows and a piece without gaps, and of any two that start alike.
+static bool meet(const Span& a, const Span& b) {
+    typedef __int128 wide;
+    if (!a.p || !b.p || a.width == 0 || b.width == 0) return false;
+    auto extent = [](const Span& s) { return (wide)(s.B - 1) * s.bs + (wide)(s.T - 1) * s.ts + s.width; };
+    auto whole = [](const Span& s) {
+        return ((s.T == 1 || s.ts == s.width) && (s.B == 1 || (wide)s.bs == (wide)s.T * s.width)) ||
+               ((s.B == 1 || s.bs == s.width) && (s.T == 1 || (wide)s.ts == (wide)s.B * s.width));
+    };
+    const wide ea = extent(a), eb = extent(b), d = (wide)(intptr_t)b.p - (intptr_t)a.p;
+    if (d >= ea || -d >= eb) return false;
+    if (d == 0) return true;
+    if (ea + eb > (wide)1 << 60) return false;  // (no device's memory)
+    if (a.bs == b.bs && a.ts == b.ts && a.B == b.B && a.T == b.T)
+        return hits(-b.width, a.width, (long long)d, 1 - a.B, a.B - 1, a.bs, 1 - a.T, a.T - 1, a.ts);
+    if (whole(a)) return hits(-b.width, (long long)ea, (long long)d, 0, b.B - 1, b.bs, 0, b.T - 1, b.ts);
+    return whole(b) && hits(-a.width, (long long)eb, (long long)-d, 0, a.B - 1, a.bs, 0, a.T - 1, a.ts);
+}
+
+int check_overlaps(const char* who, const Span& output, const char* what, std::initializer_list<Span> inputs) {
+    for (const Span& in : inputs)
+        if (meet(output, in)) {
+            set_error("%s: %s overlaps another argument of the call", who, what);
+            return MV_EINVAL;
+        }
+    return MV_OK;
+}
+
 template <typename T>
 struct NormParams {
     Rows<const T> x;
@@ -685,6 +730,12 @@ int mv_group_norm(const mv_group_norm_args* a, void* workspace, size_t workspace
     if (int rc = check_aligned("mv_group_norm", a->weight, wsize)) return rc;
     if (int rc = check_aligned("mv_group_norm", a->bias, wsize)) return rc;
     if (int rc = check_aligned("mv_group_norm", a->lengths, 4)) return rc;
+    const bool in_place = a->x.ptr == a->y.ptr && (a->B < 2 || a->x.batch_stride == a->y.batch_stride) &&
+                          (a->T < 2 || a->x.row_stride == a->y.row_stride);
+    const Span y(a->y, a->C, a->B, a->T, a->dtype), x(in_place ? mv_rows{} : a->x, a->C, a->B, a->T, a->dtype);
+    if (int rc = check_overlaps("mv_group_norm", y, "y", {x, {a->weight, a->C * (long long)wsize}, {a->bias, a->C * (long long)wsize},
+                                                          {a->lengths, 4ll * a->B}}))
+        return rc;
     const NormPlan plan = norm_plan(a);
     if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 255) != 0)) {
         set_error("mv_group_norm: workspace: need %zu bytes, 256-byte aligned (got %zu)", plan.bytes, workspace_bytes);

@@ -685,6 +685,26 @@ int mv_selective_scan(const mv_selective_scan_args* a, void* workspace, size_t w
         if (in.r != &a->z || in.r->ptr)
             if (int rc = check_rows(who, in.name, *in.r, a->T, a->dtype)) return rc;
     if (int rc = check_output_rows(who, a->y, a->B, a->T, a->D, a->dtype)) return rc;
+    auto rows = [&](const mv_rows& r, long long channels) { return Span(r, channels, a->B, a->T, a->dtype); };
+    const Span y = rows(a->y, a->D), before(a->state_in, 4 * states), after(a->state_out, 4 * states);
+    auto apart = [&](const Span& out, const char* what, std::initializer_list<Span> states_of_call) {
+        if (int rc = check_overlaps(who, out, what, states_of_call)) return rc;
+        if (int rc = check_overlaps(who, out, what, {rows(a->u, a->D), rows(a->delta, a->D), rows(a->z, a->D), {a->A, 4ll * a->D * a->N},
+                                                     {a->Dskip, 4ll * a->D}, {a->delta_bias, 4ll * a->D}, {a->lengths, 4ll * a->B}}))
+            return rc;
+        for (auto [m, step] : {std::pair<mv_rows, int64_t>{a->Bm, a->Bg_stride}, {a->Cm, a->Cg_stride}}) {
+            // all groups and what lies between them; only what touches that is looked at group by group
+            if (a->G > 1 && step > 1ll << 38) continue;  // (no device's memory, and no product of 64 bits)
+            int rc = check_overlaps(who, out, what, {rows(m, a->G == 1 ? a->N : (a->G - 1) * step + a->N)});
+            if (!rc) continue;
+            if (a->G == 1 || step == a->N) return rc;
+            for (int g = 0; g < a->G; ++g, m.ptr = (char*)m.ptr + step * (int64_t)dtype_size(a->dtype))
+                if ((rc = check_overlaps(who, out, what, {rows(m, a->N)}))) return rc;
+        }
+        return MV_OK;
+    };
+    if (int rc = apart(y, "y", {before, after})) return rc;
+    if (int rc = apart(after, "state_out", {})) return rc;
     const ScanPlan plan = scan_plan(a);
     if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 255) != 0)) {
         set_error("%s: workspace: need %zu bytes, 256-byte aligned (got %zu)", who, plan.bytes, workspace_bytes);

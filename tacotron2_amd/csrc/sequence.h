@@ -156,4 +156,17 @@ int check_rows(const char* who, const char* what, const mv_rows& r, int T, int d
 int check_states(const char* who, const void* in, const void* out, long long bytes);
 int check_output_rows(const char* who, const mv_rows& r, int B, int T, int C, int dtype);
 
+// memory of a call: B x T rows of `width` bytes (of an axis of one the stride is 0)
+struct Span {
+    const char* p;
+    long long width, bs, ts;
+    int B, T;
+    Span(const void* ptr, long long bytes) : p((const char*)ptr), width(bytes), bs(0), ts(0), B(1), T(1) {}
+    Span(const mv_rows& r, long long channels, int B_, int T_, int dtype)
+        : p((const char*)r.ptr), width(channels * (long long)dtype_size(dtype)),
+          bs(B_ > 1 ? (r.batch_stride < 1ll << 56 ? r.batch_stride : 1ll << 56) * (long long)dtype_size(dtype) : 0),
+          ts(T_ > 1 ? r.row_stride * (long long)dtype_size(dtype) : 0), B(B_), T(T_) {}
+};
+int check_overlaps(const char* who, const Span& output, const char* what, std::initializer_list<Span> inputs);
+
 }  // namespace mv

@@ -16,10 +16,10 @@ frames past the end are written as 0.  Host-side lengths outside `[0, T]` raise,
 there.
 
 `state=` is where a sequence stands before the call (None: at its beginning), `state_out=` a tensor that receives where it
-stands after its last true frame; they may be the same tensor, so a sequence cut into calls (prompt, then frame by frame)
-gives the results of one call: the convolution bit for bit, the scan to float32 rounding.  Calls can be captured into HIP
-graphs, with `lengths` on the device (host-side ones are refused there); a decode step on static tensors with its state
-replaced in place is one kernel.
+stands after its last true frame; they may be the same tensor (but share memory with no other argument), so a sequence cut
+into calls (prompt, then frame by frame) gives the results of one call: the convolution bit for bit, the scan to float32
+rounding.  Calls can be captured into HIP graphs, with `lengths` on the device (host-side ones are refused there); a decode
+step on static tensors with its state replaced in place is one kernel.
 
 These are synthesis-time layers: inputs that require a gradient are refused (outside `no_grad`), and so are those with a
 forward-mode tangent.

@@ -1005,3 +1005,30 @@ def test_lengths_of_the_host_are_refused_in_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@torch.no_grad()
+def test_results_between_the_rows_of_their_inputs():
+    """Halves of one buffer through the C entry points, [B][T] and [T][B]: y is x's other half, and x stays what it is."""
+    import ctypes
+
+    B, T, C = 3, 50, 24
+    lib, st = _native.lib(), torch.cuda.current_stream().cuda_stream
+    w = torch.randn(C, 4, generator=_rng(4)).cuda()
+    for shape, swap in (((B, T, 2 * C), False), ((T, B, 2 * C), True)):
+        buf = torch.randn(*shape, generator=_rng(5)).cuda()
+        v = buf.transpose(0, 1) if swap else buf
+        x, y = v[..., :C], v[..., C:]
+        keep, at = x.clone(), lambda t: (t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
+        a = _native.mv_causal_conv_args(*at(x), *at(y), w.data_ptr(), None, None, None, None, B, T, C, 4, 0, 0, 0, 0.0)
+        assert lib.mv_causal_conv(ctypes.byref(a), st) == 0, lib.mv_last_error()
+        assert torch.equal(y, sequence.causal_conv(keep, w)) and torch.equal(x, keep)
+        a = _native.mv_group_norm_args(*at(x), *at(y), None, None, None, B, T, C, 3, 0, 0, 0, 1, 0.0, 1e-5)
+        assert lib.mv_group_norm(ctypes.byref(a), None, 0, st) == 0, lib.mv_last_error()
+        assert torch.equal(y, sequence.group_norm(keep, 3, activation="silu")) and torch.equal(x, keep)
+    h = torch.zeros(2, 3, C, device="cuda")
+    with pytest.raises(_native.MelvocError, match="overlap"):  # the next state over the frames it comes from
+        x = torch.randn(1, 40, C, device="cuda")
+        sequence.causal_conv(x, w, state_out=x[:, 10:13])
+    with pytest.raises(_native.MelvocError, match="overlap"):
+        sequence.causal_conv(h, w, state_out=h)

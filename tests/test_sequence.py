@@ -105,3 +105,51 @@ def test_single_frames_never_need_scratch():
             a = _native.mv_selective_scan_args(P, D, D, P, D, D, None, 0, 0, P, N, N, P, N, N, 0, 0, 2 * P, D, D, P, None, None,
                                                None, None, None, B, 1, D, N, 1, 1, 1)
             assert lib.mv_selective_scan_workspace(ctypes.byref(a)) == 0
+
+
+OVERLAPS = [
+    # in place with other strides; shifted by channels, by a frame, by a sequence; rows inside the other's rows
+    (_norm, dict(y=P, y_row_stride=64, y_batch_stride=640)), (_norm, dict(y=P, y_batch_stride=384)),
+    (_norm, dict(y=P + 16)), (_norm, dict(y=P + 128)), (_norm, dict(y=P + 1280)), (_norm, dict(y=P - 2 * 1280 + 4)),
+    (_norm, dict(y=P + 124, x_row_stride=64, x_batch_stride=640, y_row_stride=64, y_batch_stride=640)),
+    (_norm, dict(y=P + 4 * 64 * 9 + 4, x_row_stride=64, x_batch_stride=640, y_row_stride=64, y_batch_stride=640)),
+    (_norm, dict(y=P + 4, x_row_stride=64, x_batch_stride=32, y_row_stride=64, y_batch_stride=32)),  # [T][B][C]
+    (_norm, dict(y=P + 256, x_row_stride=64, x_batch_stride=640)),  # strides differ, y one piece
+    (_norm, dict(y=P + 4, x_row_stride=0, x_batch_stride=0)), (_norm, dict(weight=2 * P + 64)), (_norm, dict(bias=2 * P + 2556)),
+    (_norm, dict(lengths=2 * P + 1280)),
+    (_conv, dict(y=P)), (_conv, dict(y=P + 128)), (_conv, dict(y=P - 64)), (_conv, dict(y=3 * P)), (_conv, dict(y=3 * P - 4)),
+    (_conv, dict(state_in=None, state_out=P + 128)), (_conv, dict(state_in=None, state_out=2 * P + 2556)),
+    (_conv, dict(state_in=None, state_out=P - 2 * 384 + 4)), (_conv, dict(weight=2 * P)), (_conv, dict(bias=3 * P)),
+    (_conv, dict(state_in=None, state_out=P + 128 + 4, x_row_stride=64, x_batch_stride=640, B=1)),
+    (_scan, dict(y=P)), (_scan, dict(y=P + 8, z=2 * P, z_batch_stride=320, z_row_stride=32)), (_scan, dict(y=3 * P)),
+    (_scan, dict(y=P + 64, Bm=5 * P, Cm=P + 128)), (_scan, dict(Bm=2 * P + 2556)), (_scan, dict(Cm=2 * P, Cm_row_stride=0)),
+    (_scan, dict(G=2, N=16, Bg_stride=2 ** 18, Bm=P)),  # only the second group of B lies in y
+    (_scan, dict(A=2 * P)), (_scan, dict(Dskip=2 * P + 128)), (_scan, dict(delta_bias=3 * P)), (_scan, dict(A=3 * P + 4092)),
+    (_scan, dict(state_in=None, state_out=P)), (_scan, dict(state_in=None, state_out=2 * P - 4)), (_scan, dict(delta=3 * P + 64)),
+]
+
+
+@pytest.mark.parametrize("call,fields", OVERLAPS)
+def test_outputs_over_inputs_are_refused(call, fields):
+    assert call(**fields) == -1
+    assert b"overlap" in _native.lib().mv_last_error(), _native.lib().mv_last_error()
+
+
+def test_outputs_beside_inputs_are_not():
+    """Rows that lie between the other's rows get past the checks: what then stops these calls is that they bring no scratch."""
+    T = 100000
+    for x, y, b, r in ((P, P + 128, 64 * T, 64), (P + 128, P, 64 * T, 64), (P, P + 128, 64, 128), (P, P + 4 * 64 * T, 32 * T, 32),
+                       (P, P, 32 * T, 32)):  # halves of rows, also of [T][B] memory; one behind the other; in place
+        rows = dict(x=x, x_batch_stride=b, x_row_stride=r, y=y, y_batch_stride=b, y_row_stride=r, weight=None, bias=None)
+        assert _norm(T=T, **rows) == -4, _native.lib().mv_last_error()
+    T = 5000
+    far = P + 8 * 160 * T  # behind both sequences' rows
+    scan = dict(T=T, delta=far, delta_batch_stride=32 * T, A=2 * far, Dskip=None, delta_bias=None, state_in=3 * far, state_out=3 * far)
+    # u, B, C and y side by side in rows of 160: the groups of B and C 32 apart, y between them
+    side = dict(u=P, u_batch_stride=160 * T, u_row_stride=160, G=2, N=16, Bm=P + 4 * 32, Bm_batch_stride=160 * T, Bm_row_stride=160,
+                Bg_stride=64, Cm=P + 4 * 48, Cm_batch_stride=160 * T, Cm_row_stride=160, Cg_stride=64, y_batch_stride=160 * T,
+                y_row_stride=160)
+    for y in (64, 128):
+        assert _scan(**scan, **side, y=P + 4 * y) == -4, _native.lib().mv_last_error()
+    for y in (1, 33, 65, 80, 127):
+        assert _scan(**scan, **side, y=P + 4 * y) == -1 and b"overlap" in _native.lib().mv_last_error()
