@@ -474,10 +474,12 @@ __global__ __launch_bounds__(256) void frame_norm_kernel(NormParams<T> p, int L,
     }
 }
 
-// One block per group of a sequence (or of a frame), element by element: groups that no block's registers hold.
+// One block per group of a sequence (or of a frame), element by element: groups that no block's registers hold.  A thread's sums
+// run over all frames, so they are held in 64 bits: a chain of float32 additions loses as many roundings as it has terms (the mean
+// of 300 x 10000 values near 3, spread 0.01, was off by enough for 1.3 times the error of a rounded one in the result).
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void wide_norm_kernel(NormParams<T> p, int per_frame) {
-    __shared__ float red[256];
+    __shared__ double red[256];
     const int Cg = p.C / p.G;
     long long item = blockIdx.x;
     const int g = item % p.G;
@@ -489,35 +491,29 @@ __global__ __launch_bounds__(256) void wide_norm_kernel(NormParams<T> p, int per
         item /= p.Tmax;
     }
     const int b = (int)item, len = seq_frames(p.lengths, b, p.Tmax), c0 = g * Cg, end = min(t1, len);
-    const float count = (float)max(0, end - t0) * (float)Cg;
-    auto total = [&](float v) {
+    const double count = (double)max(0, end - t0) * (double)Cg;
+    auto total = [&](double v) {
         red[threadIdx.x] = v;
         __syncthreads();
         for (int s = 128; s; s >>= 1) {
             if (threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
             __syncthreads();
         }
-        const float r = red[0];
+        const double r = red[0];
         __syncthreads();
         return r;
     };
-    float s = 0.f;
-    for (int t = t0; t < end; ++t) {
-        float row = 0.f;  // (a row's sum by itself: a thread adds up at most its channels plus its rows in one chain)
-        for (int c = threadIdx.x; c < Cg; c += 256) row += (float)p.x.row(b, t)[c0 + c];
-        s += row;
-    }
-    const float mean = total(s) / count;
-    s = 0.f;
-    for (int t = t0; t < end; ++t) {
-        float row = 0.f;
+    double s = 0.;
+    for (int t = t0; t < end; ++t)
+        for (int c = threadIdx.x; c < Cg; c += 256) s += (float)p.x.row(b, t)[c0 + c];
+    const float mean = (float)(total(s) / count);
+    s = 0.;
+    for (int t = t0; t < end; ++t)
         for (int c = threadIdx.x; c < Cg; c += 256) {
             const float d = (float)p.x.row(b, t)[c0 + c] - mean;
-            row += d * d;
+            s += d * d;
         }
-        s += row;
-    }
-    const float rstd = 1.f / sqrtf(total(s) / count + p.eps);
+    const float rstd = 1.f / sqrtf((float)(total(s) / count) + p.eps);
     for (int t = t0; t < t1; ++t)
         for (int c = c0 + threadIdx.x; c < c0 + Cg; c += 256) {
             float v = 0.f;

@@ -1032,3 +1032,26 @@ def test_results_between_the_rows_of_their_inputs():
         sequence.causal_conv(x, w, state_out=x[:, 10:13])
     with pytest.raises(_native.MelvocError, match="overlap"):
         sequence.causal_conv(h, w, state_out=h)
+
+
+@pytest.mark.parametrize("T,C,G,per_frame,dtype", [(4000, 5000, 1, False, F32), (300, 20000, 2, False, F32), (5, 300001, 1, True, F32),
+                                                   (2500, 8200, 1, False, F16)])
+def test_group_norm_of_wide_groups_adds_up_many_rows(T, C, G, per_frame, dtype):
+    """Values near 3, spread 0.01: an error of k u in the mean (relative) shows as 300 k u in the result.  The sums are held
+    in 64 bits, so the mean is off by its own rounding, u of itself, and the distances by u of theirs; 1 / sqrt(var + eps) is
+    off by 4 u (rounded variance, sum with eps, root, reciprocal) and what the mean's error adds to the variance."""
+    x = (3 + 0.01 * torch.randn(2, T, C, generator=_rng(T))).to(dtype)
+    ends = [T, T - T // 3]
+    y = sequence.group_norm(x.cuda(), G, per_frame=per_frame, lengths=_on(ends)).cpu()
+    for i, end in enumerate(ends):
+        v = x[i, :end].double().view(end, G, C // G)
+        dims = (2,) if per_frame else (0, 2)
+        m = v.mean(dims, keepdim=True)
+        var = ((v - m) ** 2).mean(dims, keepdim=True)
+        r = 1 / torch.sqrt(var + 1e-5)
+        em = U * m.abs()
+        d = v - m
+        er = r * (4 * U + 0.5 * em * em * r * r)
+        err = (em + U * (d.abs() + em)) * r + d.abs() * er + 3 * U * (d * r).abs()
+        _near(y[i, :end], (d * r).view(end, C), err.reshape(end, C))
+        assert not y[i, end:].any()
