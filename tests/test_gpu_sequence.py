@@ -1055,3 +1055,33 @@ def test_group_norm_of_wide_groups_adds_up_many_rows(T, C, G, per_frame, dtype):
         err = (em + U * (d.abs() + em)) * r + d.abs() * er + 3 * U * (d * r).abs()
         _near(y[i, :end], (d * r).view(end, C), err.reshape(end, C))
         assert not y[i, end:].any()
+
+
+@pytest.mark.parametrize("N", [23, 32])
+@pytest.mark.parametrize("T", [45, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_selective_scan_of_17_to_32_states(N, T, dtype):
+    """Eight states to a lane: whole (45 frames of enough sequences) and in pieces."""
+    p = scan_inputs(3, T, 70, N, 2, dtype, True, True, N + T)
+    ends = [T, T // 3, T - 1]
+    for i, end in enumerate(ends):
+        for k in ("u", "delta", "Bm", "Cm", "z"):
+            p[k][i, end:] = float("nan")
+    out = torch.empty(3, 70, N, device="cuda")
+    y = scan_run(p, True, _on(ends), out)
+    want, err, h, eh = scan_ref(softplus=True, ends=ends, **p)
+    _near(y, want, err, "y")
+    _near(out, h, eh, "state")
+
+
+@pytest.mark.parametrize("B,T,D", [(40, 70, 512), (40, 33, 1024), (7, 12, 8192), (33, 40, 500)])
+def test_selective_scan_of_padded_batches_in_more_than_one_round(B, T, D):
+    """More sequences than fill the CUs once (256 / 64-channel blocks of them), so the longest-first order has backward and
+    partial rounds; with equal lengths and empty sequences."""
+    p = scan_inputs(B, T, D, 4, 1, BF16, False, True, B + D)
+    ends = [(7 * i) % (T + 1) if i % 4 else (T, 0, T // 2)[i // 4 % 3] for i in range(B)]
+    out = torch.full((B, D, 4), 7.0, device="cuda")
+    y = scan_run(p, True, _on(ends), out)
+    want, err, h, eh = scan_ref(softplus=True, ends=ends, **p)
+    _near(y, want, err, "y")
+    _near(out, h, eh, "state")
