@@ -4,21 +4,23 @@
 //
 // HBM-bound: x once in, y once out.  The variance is a sum of squared distances from a mean that is already known (sums of
 // squares lose it where the mean is far from zero), so what is normalised has to be looked at twice: it stays in registers
-// between the two looks wherever it fits.  32 utterances of up to 861 frames, 512 channels, 32 groups, bf16, SiLU: 12.8 us
-// (3.5 TB/s, all in one load and one store phase a block); 16 of up to 55104 x 128, float16, in pieces: 97 us (statistics 33, the
-// second pass 67 at 5.5 TB/s); 64 single frames of 1024 channels: 3.6 us, a launch.
+// between the two looks wherever it fits.  32 utterances of up to 861 frames, 512 channels, 32 groups, bf16, SiLU: 12.9 us
+// (3.5 TB/s, all in one load and one store phase a block); 16 of up to 55104 x 128, float16, in pieces: 95 - 99 us (statistics 33,
+// the second pass 68 at 5.4 TB/s); 64 single frames of 1024 channels: 3.6 us, a launch.
 //
 //   frame_norm_kernel     per frame, groups of up to 64 * 8 vectors: L lanes hold a group
 //   group_norm_kernel     a sequence's group(s) in one block's registers: one read, one write, one launch
 //   group_stats_kernel +  a sequence in pieces: count, mean and squared distances of each, batch by batch; then the pieces are
 //   group_apply_kernel    put together and x is read a second time
-//   wide_norm_kernel      what none of them holds: groups of more channels than a block holds at once
+//   wide_norm_kernel      what none of them holds: groups of more channels than a block holds at once, one block to a group and
+//                         one element to a load, three times over x (a sequence of 500 x 8200 float32, one group: 13.7 ms, where
+//                         500 x 4096 take 16 us; 8 x 861 frames of 8200 bf16 channels, a group each, 129 us)
 //
 // A vector is as many channels of a group as there are, a power of two of them, 16 bytes at most, at any address.  It never
 // holds two groups: where the group is no multiple of it (R), the group's last vector reaches back over the one before; what
-// both hold counts once (`skip`), and both write the same.  32 x 861 frames, bf16, C about 512: groups of 17 channels 26 us
+// both hold counts once (`skip`), and both write the same.  32 x 861 frames, bf16, C about 512: groups of 17 channels 25 us
 // and per frame 24 us (31 and 111 us with the largest vector that divides the group, one channel), of 7 20 and 20 us (59 and
-// 60 us), of 16, where nothing overlaps, 15 and 14 us; a group of one channel, a vector of its own, 78 us.
+// 60 us), of 16, where nothing overlaps, 15 and 14 us; a group of one channel, a vector of its own, 78 - 99 us.
 #include "sequence.h"
 
 namespace mv {

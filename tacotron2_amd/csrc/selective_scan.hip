@@ -2,13 +2,15 @@
 //
 //   h[n] = exp(dt A[d, n]) h[n] + dt u B[g, n],   y = (sum_n C[g, n] h[n] + D u) z sigmoid(z)
 //
-// What bounds it.  Many frames: the vector unit.  A state costs an exponential (8.6 cycles of a SIMD, measured), the product in
-// its argument and two multiply-adds (2.9 each with two waves on the SIMD, 4 - 5 with one): 17 cycles for 64 states against
-// 8 bytes a channel and frame, so 16 states of 1024 channels take twice what their bytes would.  What is left of the unit goes
-// to the steps' softplus, the gate and the sums over states.  Frames of a channel are a chain: the parallelism is sequences x
-// channels, four lanes to a channel (scan_kernel), and pieces of the frames where that does not fill the chip, at the price of
-// going through them twice (a piece's decay needs no more than its sum of dt: exp(A sum dt)).  32 utterances of 172 - 861
-// frames, 1024 channels, 16 states, bf16: 94 us; one of 8192 frames: 75 us.
+// What bounds it.  Many frames: the vector unit.  A wave issues 27.3 vector instructions for a frame of 16 channels x 16 states,
+// 5.0 of them transcendental (the states' exponentials are 4), and the counters show the unit active for 132 cycles of it (they
+// count 4 for an instruction, 8 for a transcendental) while the CU is busy for 170.  With two waves on a SIMD, each spends 55 %
+// of its life issuing, 24 % waiting to issue and 20 % for data, and the two blocks of a CU do not end together (a wave lives 86 %
+// of the time its CU is busy).  32 utterances of 861 frames, 1024 channels, 16 states, bf16: 130 us, 73 ns a wave's frame (the
+// bytes take 45 us); padded ones of 172 - 861 frames: 94 us a call, where that rate alone would give 77.  Frames of a channel are a chain: the parallelism is sequences x channels, four lanes to a channel (scan_kernel), and
+// pieces of the frames where that does not fill the chip, at the price of going through them twice (a piece's decay needs no
+// more than its sum of dt: exp(A sum dt)).  One sequence of 8192 frames: 76 us, 32 for the first launch (piece 0, whose results
+// it makes, takes all of that) and 49 for the second.
 // One frame of many sequences: the state, in and out once (scan_step_kernel).  512 sequences, 71 MB: 17.8 us, 4.0 TB/s.
 #include "sequence.h"
 
@@ -401,7 +403,7 @@ __device__ __forceinline__ float* piece_sum(const ScanParams<T>& p, const Channe
 
 // The sequence that the block at place z takes: by falling length, every second round of `order` places backwards.  A round is
 // what fills the CUs once, so that the block that comes second to a CU has the shorter sequence the longer the first one's
-// is.  (32 utterances of 172 to 861 frames, D 1024: 89 us; as they come 114 - 125 us.)
+// is.  (32 utterances of 172 to 861 frames, D 1024: 94 - 98 us; as they come 118.)
 __device__ __forceinline__ int place_to_sequence(const int32_t* lengths, int B, int Tmax, int order, int z, int* found) {
     const int round = z / order, first = round * order;
     const int rank = round & 1 ? first + min(order, B - first) - 1 - (z - first) : z;
@@ -576,12 +578,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams<T> p) {
 constexpr int kStepBlocks = 2048;  // of the step kernel: eight to a CU, each then walks B * D / 64 / 2048 sequences
 
 // Calls of up to this many frames take the step kernel, whose frames cost their own memory instructions; the other one computes
-// 16 at a time (D 1024, 64 / 512 sequences: 8 frames 11.2 / 38.5 us against 14.0 / 91; 16 frames of 64 sequences 17.3 against 14).
+// 16 at a time (D 1024, 64 / 512 sequences: 8 frames 12.2 / 40 us against 14.5 / 91; 16 frames of 64 sequences 21.6 against 14.5).
 constexpr int kStepFrames = 8;
 
 // Pieces that the frames of each sequence are cut into: as many as give every SIMD two waves (which is what the registers
-// hold), of 32 frames at least.  The work doubles, so two pieces gain nothing (1 x 8192 frames, D 1024: 111 us with waves for
-// one a SIMD, 81 for two, 92 for three or four; 8 x 861: 70 cut in four, 86 whole; 12 x 861: 86 whole, 100 in three), and a
+// hold), of 32 frames at least.  The work doubles, so two pieces gain nothing (1 x 8192 frames, D 1024: 109 us with waves for
+// one a SIMD, 76 for two, 88 - 90 for three or four; 8 x 861: 71 cut in four, 87 whole; 12 x 861: 87 whole, 92 in three), and a
 // launch takes what 30 frames take (1 x 861, D 256: 17.9 us in 27 pieces of 32, 21.7 in 14 of 64).
 static int scan_pieces(int B, int T, int D, int G) {
     const long long waves = (long long)B * G * ((D / G + 15) / 16);

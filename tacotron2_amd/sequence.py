@@ -6,7 +6,8 @@ beside this package's convolutions needs and the reference's models do not hold.
     y = selective_scan(u, delta, A, B, C, D=D, z=z, state=h, state_out=h)           # state space recurrence
 
 Data are `[B, T, channels]` float32, bfloat16 or float16 with adjacent channels and any other strides (halves of a
-projection's output, `[T, B, C]` memory: taken as they lie; a tensor whose channels are not adjacent is copied first).  A
+projection's output, `[T, B, C]` memory: taken as they lie, rows at most 2^25 elements apart; a tensor whose channels are not
+adjacent is copied first).  A
 tensor without the frame axis, `[B, channels]`, is one frame of each sequence: a decode step.  Arithmetic is float32 and is
 rounded once, at the result.
 
